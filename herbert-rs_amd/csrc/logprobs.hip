@@ -1,0 +1,284 @@
+// What a step's logits say of given tokens: for every row x of V logits and its token t
+//   log p(t) = x_t - m - log S,   S = sum e^(x - m),   m = max x,
+//   entropy  = log S - T / S,     T = sum (x - m) e^(x - m)   (-inf: e^-inf = 0, and 0 (-inf) counts as 0),
+// and the `top` largest logits with their log p, larger first and the lower id first among equals.
+//
+// Bound by reading the logits once. A row is cut into chunks of 4,096, a workgroup of 256 threads each, which holds its chunk in
+// registers (16 a thread), finds its (m, S, T) and its own `top` largest; a second kernel adds a row's chunks up:
+//   S = sum S_c e^(m_c - m),   T = sum (T_c + (m_c - m) S_c) e^(m_c - m).
+// A row of one chunk needs no second kernel.
+// The reference computes a softmax on the host to draw a token (crates/core/src/sampler.rs:72-145) and reports no
+// probabilities.
+#include "common.h"
+#include <math.h>
+#include <type_traits>
+
+HB_MODULE_ERROR_SLOT()
+
+#define CHUNK 4096
+#define THREADS 256
+#define PER (CHUNK / THREADS)
+#define MAX_TOP 64
+#define LISTED 1024        // candidates that are ranked at once
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+
+// A logit and its id as one number, larger for what comes first: the value's order in the upper half, the id's complement
+// in the lower one. 0 is none (a NaN's key is as good as any: such a row is refused as a whole).
+__device__ __forceinline__ uint64_t key_of(float v, int id) {
+    const uint32_t u = __float_as_uint(v == 0.f ? 0.f : v);       // (-0 equals 0)
+    return ((uint64_t)((u & 0x80000000u) ? ~u : (u | 0x80000000u)) << 32) | (uint32_t)~id;
+}
+__device__ __forceinline__ int id_of(uint64_t key) { return (int)~(uint32_t)key; }
+__device__ __forceinline__ float value_of(uint64_t key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
+}
+
+// e^u for u <= 0 by the hardware's power of two; the rounding of u log2 e, which grows with |u|, is put back.
+__device__ __forceinline__ float exp_of(float u) {
+    const float t = u * 1.44269502f;
+    const float left = fmaf(u, 1.44269502f, -t) + u * 1.92596303e-8f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    return u > -150.f ? fmaf(e * left, 0.693147182f, e) : e;
+}
+
+__device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int off) {
+    const uint32_t lo = __shfl_xor((int)(uint32_t)v, off, 64), hi = __shfl_xor((int)(uint32_t)(v >> 32), off, 64);
+    return ((uint64_t)hi << 32) | lo;
+}
+
+struct Selecting {
+    uint64_t list[LISTED];
+    uint64_t groups[64], bound, wave_best[THREADS / 64];
+    int count;
+};
+
+// The `top` largest of the keys that `each(f)` hands to f one after the other (as the thread's own, key by key), written by
+// put(rank, key): ranks 0 .. top - 1, those that there is no key for with the key 0. largest: the thread's own largest key.
+// The n-th largest of the 64 largest keys of four threads each bounds the n largest of all from below, and few keys lie at or above it: those
+// are listed and ranked by counting. Where more are than the list holds, the largest is looked for `top` times.
+template <class Each, class Put>
+__device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, Put put) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    uint64_t g = largest;
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) {
+        const uint64_t o = shfl_xor_u64(g, off);
+        g = o > g ? o : g;
+    }
+    if ((tid & 3) == 0) sh.groups[tid >> 2] = g;
+    if (tid == 0) sh.count = 0, sh.bound = 0;
+    __syncthreads();
+    if (tid < 64) {
+        const uint64_t mine = sh.groups[lane];
+        int above = 0;
+        for (int i = 0; i < 64; ++i) above += sh.groups[i] > mine ? 1 : 0;
+        if (above == top - 1 && mine != 0) sh.bound = mine;        // (keys are of different ids, only 0 may be there twice)
+    }
+    __syncthreads();
+    const uint64_t bound = sh.bound > 1 ? sh.bound : 1;
+    each([&](uint64_t key) {
+        if (key >= bound) {
+            const int at = atomicAdd(&sh.count, 1);
+            if (at < LISTED) sh.list[at] = key;
+        }
+    });
+    __syncthreads();
+    const int count = sh.count;
+    if (count <= LISTED) {
+        for (int i = tid; i < count; i += THREADS) {
+            const uint64_t mine = sh.list[i];
+            int above = 0;
+            for (int j = 0; j < count; ++j) above += sh.list[j] > mine ? 1 : 0;
+            if (above < top) put(above, mine);
+        }
+        for (int i = count + tid; i < top; i += THREADS) put(i, (uint64_t)0);
+        return;
+    }
+    uint64_t before = ~(uint64_t)0;
+    for (int n = 0; n < top; ++n) {
+        uint64_t best = 0;
+        each([&](uint64_t key) { best = key < before && key > best ? key : best; });
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) {
+            const uint64_t o = shfl_xor_u64(best, off);
+            best = o > best ? o : best;
+        }
+        if (lane == 0) sh.wave_best[tid >> 6] = best;
+        __syncthreads();
+        best = sh.wave_best[0];
+        for (int w = 1; w < THREADS / 64; ++w) best = sh.wave_best[w] > best ? sh.wave_best[w] : best;
+        __syncthreads();
+        if (tid == 0) put(n, best);
+        before = best;
+    }
+}
+
+// A row's results from its m, S and T: what the row's threads share.
+struct Row {
+    float m, log_s;
+    bool bad;            // NaN or +inf among the logits, or nothing above -inf: no distribution
+};
+__device__ __forceinline__ Row row_of(float m, float S) {
+    Row r;
+    r.m = m;
+    r.bad = !(S > 0.f && S < INFINITY);
+    r.log_s = logf(S);
+    return r;
+}
+__device__ __forceinline__ void leave_token(const Row& r, float S, float T, const float* row, int V, int token, float* chosen,
+                                            float* entropy) {
+    const float nan = __uint_as_float(0x7fc00000u);
+    *chosen = r.bad || token < 0 || token >= V ? nan : (row[token] - r.m) - r.log_s;
+    *entropy = r.bad ? nan : fmaxf(r.log_s - T / S, 0.f);
+}
+__device__ __forceinline__ void leave_top(const Row& r, uint64_t key, int* id, float* best) {
+    *id = r.bad ? -1 : id_of(key);
+    *best = r.bad ? __uint_as_float(0x7fc00000u) : (value_of(key) - r.m) - r.log_s;
+}
+
+// stats [row][chunk]: (m, S, T); keys [row][chunk][top]. One chunk a row: the row's results themselves.
+template <bool TOP>
+__global__ void __launch_bounds__(THREADS)
+logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restrict__ tokens, float* __restrict__ chosen,
+                     float* __restrict__ entropy, int* __restrict__ ids, float* __restrict__ best, int top, int chunks,
+                     float4* __restrict__ stats, uint64_t* __restrict__ keys) {
+    __shared__ float red[3][THREADS / 64];
+    __shared__ std::conditional_t<TOP, Selecting, int> sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t r = blockIdx.x / chunks;
+    const int chunk = blockIdx.x % chunks, first = chunk * CHUNK, len = V - first < CHUNK ? V - first : CHUNK;
+    const float* row = logits + r * V;
+    float x[PER];
+#pragma unroll
+    for (int j = 0; j < PER / 4; ++j) {
+        const int at = (j * THREADS + tid) * 4;
+        if (at + 4 <= len) {
+            const f32x4u v = *(const f32x4u*)(row + first + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * j + e] = v[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * j + e] = at + e < len ? row[first + at + e] : -INFINITY;
+        }
+    }
+    float m = -INFINITY;
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        m = fmaxf(m, x[i]);
+        nan |= x[i] != x[i];
+    }
+    m = hb_wave_max(m);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float S = 0.f, T = 0.f;
+    if (m != -INFINITY) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const float u = x[i] - m, e = exp_of(u);
+            S += e;
+            T += e > 0.f ? e * u : 0.f;
+        }
+    }
+    if (nan) S = __uint_as_float(0x7fc00000u);
+    S = hb_wave_sum(S);
+    T = hb_wave_sum(T);
+    if (lane == 0) red[1][wave] = S, red[2][wave] = T;
+    __syncthreads();
+    S = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    T = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+    const Row whole = row_of(m, S);
+    if (tid == 0) {
+        if (chunks > 1) stats[r * chunks + chunk] = make_float4(m, S, T, 0.f);
+        else leave_token(whole, S, T, row, V, tokens[r], chosen + r, entropy + r);
+    }
+    if constexpr (TOP) {
+        auto key_at = [&](int i) {
+            const int at = ((i >> 2) * THREADS + tid) * 4 + (i & 3);
+            return at < len ? key_of(x[i], first + at) : (uint64_t)0;
+        };
+        uint64_t largest = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint64_t k = key_at(i);
+            largest = k > largest ? k : largest;
+        }
+        select_top(sh, top, largest, [&](auto f) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) f(key_at(i));
+        }, [&](int rank, uint64_t key) {
+            if (chunks > 1) keys[(r * chunks + chunk) * top + rank] = key;
+            else leave_top(whole, key, ids + r * top + rank, best + r * top + rank);
+        });
+    }
+}
+
+// A workgroup a row: its chunks added up, in a fixed order.
+template <bool TOP>
+__global__ void __launch_bounds__(THREADS)
+logprob_row_kernel(const float* __restrict__ logits, int V, const int* __restrict__ tokens, float* __restrict__ chosen,
+                   float* __restrict__ entropy, int* __restrict__ ids, float* __restrict__ best, int top, int chunks,
+                   const float4* __restrict__ stats, const uint64_t* __restrict__ keys) {
+    __shared__ float red[3][THREADS / 64];
+    __shared__ std::conditional_t<TOP, Selecting, int> sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const size_t r = blockIdx.x;
+    stats += r * chunks;
+    float m = -INFINITY;
+    for (int c = tid; c < chunks; c += THREADS) m = fmaxf(m, stats[c].x);
+    m = hb_wave_max(m);
+    if (lane == 0) red[0][wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    float S = 0.f, T = 0.f;
+    for (int c = tid; c < chunks; c += THREADS) {
+        const float4 s = stats[c];
+        if (s.x == -INFINITY) {
+            S += s.y;                      // nothing, or NaN
+            continue;
+        }
+        const float down = s.x - m, e = exp_of(down);
+        S = fmaf(e, s.y, S);
+        if (e > 0.f) T = fmaf(e, fmaf(down, s.y, s.z), T);
+    }
+    S = hb_wave_sum(S);
+    T = hb_wave_sum(T);
+    if (lane == 0) red[1][wave] = S, red[2][wave] = T;
+    __syncthreads();
+    S = (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]);
+    T = (red[2][0] + red[2][1]) + (red[2][2] + red[2][3]);
+    const Row whole = row_of(m, S);
+    if (tid == 0) leave_token(whole, S, T, logits + r * V, V, tokens[r], chosen + r, entropy + r);
+    if constexpr (TOP) {
+        keys += r * chunks * top;
+        const int n = chunks * top;
+        uint64_t largest = 0;
+        for (int i = tid; i < n; i += THREADS) largest = keys[i] > largest ? keys[i] : largest;
+        select_top(sh, top, largest, [&](auto f) {
+            for (int i = tid; i < n; i += THREADS) f(keys[i]);
+        }, [&](int rank, uint64_t key) { leave_top(whole, key, ids + r * top + rank, best + r * top + rank); });
+    }
+}
+
+// logits [R, V], tokens [R] -> chosen [R], entropy [R]; top > 0: ids, best [R, top]. stats: 4 floats for every row and chunk of 4,096, keys: 2
+// floats' room for every one of their `top` (both only for V > 4,096).
+extern "C" int hb_token_logprobs(const float* logits, int R, int V, const int* tokens, float* chosen, float* entropy, int* ids,
+                                 float* best, int top, void* stats, void* keys, hipStream_t stream) {
+    HB_REQUIRE(R > 0 && V > 0 && top >= 0 && top <= MAX_TOP && top <= V, "log probabilities: bad sizes (R=%d, V=%d, top=%d)", R, V, top);
+    const int chunks = (V - 1) / CHUNK + 1;
+    HB_REQUIRE((long long)R * chunks <= 0x7fffffffLL, "log probabilities: too many rows for the grid");
+    HB_REQUIRE(chunks == 1 || (stats && (top == 0 || keys)), "log probabilities: rows of more than %d logits need room for their chunks", CHUNK);
+    const unsigned grid = (unsigned)(R * chunks);
+    if (top > 0) logprob_chunk_kernel<true><<<grid, THREADS, 0, stream>>>(logits, V, tokens, chosen, entropy, ids, best, top, chunks, (float4*)stats, (uint64_t*)keys);
+    else logprob_chunk_kernel<false><<<grid, THREADS, 0, stream>>>(logits, V, tokens, chosen, entropy, ids, best, top, chunks, (float4*)stats, (uint64_t*)keys);
+    HB_CHECK_LAUNCH("log probabilities");
+    if (chunks > 1) {
+        if (top > 0) logprob_row_kernel<true><<<R, THREADS, 0, stream>>>(logits, V, tokens, chosen, entropy, ids, best, top, chunks, (const float4*)stats, (const uint64_t*)keys);
+        else logprob_row_kernel<false><<<R, THREADS, 0, stream>>>(logits, V, tokens, chosen, entropy, ids, best, top, chunks, (const float4*)stats, (const uint64_t*)keys);
+        HB_CHECK_LAUNCH("log probabilities: rows");
+    }
+    return 0;
+}

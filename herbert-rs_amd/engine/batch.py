@@ -44,6 +44,7 @@ class BatchMeta:
     unequal: int = 0           # how unequal the contexts' lengths are: 0 (alike), 1, 2 (see unequal_level)
     num_real: int = 0          # sequences that are no padding rows (0: all of them)
     static: object = None      # the StaticDecodeMeta whose buffers these are, if any
+    shared: object = None      # the pages that sequences of this step hold together (cache.SharedPages); None: none
 
     def ranges_for(self, items, unit):
         """The list that cuts this step's contexts into at most `items` ranges of equally many whole

@@ -102,6 +102,9 @@ SIGNATURES = {
         "hb_force_tokens": [_P, _I, _I, _I, _P, _P, _I, _P],
         "hb_sample_all": [_P, _I, _I, _I, _F, _P, _P, _P, _P, _P],
     },
+    "logprobs": {
+        "hb_token_logprobs": [_P, _I, _I, _P, _P, _P, _P, _P, _I, _P, _P, _P],
+    },
 }
 
 

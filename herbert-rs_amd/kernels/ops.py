@@ -421,6 +421,52 @@ def force_tokens(logits, rows, tokens):
              len(rows), _stream())
 
 
+LOGPROB_CHUNK = 4096
+LOGPROB_MOST = 64            # alternatives a row
+
+
+def logprob_scratch(rows, vocab, top, device):
+    """What `token_logprobs` needs for up to `rows` rows of `vocab` logits and `top` alternatives, to be kept and handed to it again and
+    again: (statistics float32, candidates int64), or None for rows that it takes whole."""
+    chunks = -(-vocab // LOGPROB_CHUNK)
+    if chunks == 1:
+        return None
+    return (torch.empty(rows * chunks * 4, dtype=torch.float32, device=device),
+            torch.empty(max(1, rows * chunks * top), dtype=torch.int64, device=device))
+
+
+def token_logprobs(logits, tokens, chosen, entropy, ids=None, best=None, scratch=None):
+    """chosen[r] = log p(tokens[r]) and entropy[r] = -sum p log p of the softmax of logits[r]; ids[r], best[r]: the row's largest
+    entries and their log p, larger first, the lower id first among equals. logits f32 [R, V], tokens int32 [R] (one outside the
+    vocabulary: NaN), chosen, entropy f32 [R], ids int32 and best f32 [R, n] with n <= 64 (both or neither). A
+    row that holds NaN or +inf, or nothing above -inf, is no distribution: NaN, and the ids are -1.
+    `scratch` as `logprob_scratch` makes it (for at least R such rows), else it is allocated here."""
+    _check(logits, "logits", torch.float32, (None, None))
+    R, V = logits.shape
+    _check(tokens, "tokens", torch.int32, (R,))
+    _check(chosen, "chosen", torch.float32, (R,))
+    _check(entropy, "entropy", torch.float32, (R,))
+    if (ids is None) != (best is None):
+        raise BackendError("token_logprobs: alternatives come as ids and log probabilities together")
+    top = 0
+    if ids is not None:
+        _check(ids, "ids", torch.int32, (R, None))
+        top = ids.shape[1]
+        _check(best, "best", torch.float32, (R, top))
+        if not 0 < top <= min(LOGPROB_MOST, V):
+            raise BackendError(f"token_logprobs: 1 to {min(LOGPROB_MOST, V)} alternatives of {V} logits, not {top}")
+    chunks = -(-V // LOGPROB_CHUNK)
+    stats = keys = None
+    if chunks > 1:
+        stats, keys = scratch if scratch is not None else logprob_scratch(R, V, top, logits.device)
+        _check(stats, "statistics", torch.float32, (None,))
+        _check(keys, "candidates", torch.int64, (None,))
+        if stats.numel() < R * chunks * 4 or keys.numel() < R * chunks * top:
+            raise BackendError("token_logprobs: the scratch is too small for these logits")
+    lib.call("logprobs", "hb_token_logprobs", logits.data_ptr(), R, V, tokens.data_ptr(), chosen.data_ptr(), entropy.data_ptr(),
+             _ptr(ids), _ptr(best), top, _ptr(stats), _ptr(keys), _stream())
+
+
 def layernorm(x, weight, out, eps, rows=None, delta=None, mult=1.0):
     """out[r] = (x[r] - mean) / sqrt(var + eps) * weight, var the mean of the squared deviations; x f32
     [T, H] (rows int32: only these, gathered), out f32 or the compute dtype, and it may be x itself.

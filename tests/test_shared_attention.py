@@ -1,0 +1,161 @@
+"""Which pages sequences share, how a step is cut into items, and what the shared attention refuses (no GPU needed)."""
+import numpy as np
+import pytest
+import torch
+
+from herbert_rs_amd.cache import LayerKV, shared_pages
+from herbert_rs_amd.cache.sharing import MAX_LEVELS
+from herbert_rs_amd.engine import StepEntry, batch
+from herbert_rs_amd.errors import BackendError
+from herbert_rs_amd.kernels import lib, shared
+
+from .shared_util import tables
+
+
+def as_sets(found, table, held):
+    """{sequence: [(page, end, the sequences that share it), ...]} with every page of every sequence in exactly one node."""
+    got = {}
+    for first, count, page, end in found.nodes:
+        members = sorted(int(i) for i in found.order[first:first + count])
+        for i in members:
+            got.setdefault(i, []).append((page, end, tuple(members)))
+    for i, nodes in got.items():
+        at = 0
+        for page, end, members in nodes:
+            assert page == at and (end > page or end == -1)
+            if end >= 0:
+                assert len(members) > 1 and end <= held[i] // 64
+                for j in members:
+                    assert (table[i, page:end] == table[j, page:end]).all()
+            else:
+                assert members == (i,)
+            at = end
+        assert at == -1
+    return got
+
+
+def test_sequences_that_share_pages_are_found():
+    # two branches of a common beginning, one of them with a branch of its own, and a sequence that shares nothing
+    seqs = [[("a", 3), ("b", 2), (None, 2)], [(None, 4)], [("a", 3), ("c", 1), (None, 1)], [("a", 3), ("b", 2), (None, 1)],
+            [("a", 3), ("c", 1), ("d", 2), (None, 1)], [("a", 3), ("c", 1), ("d", 2), (None, 3)]]
+    table, _ = tables(seqs, 1)
+    held = [64 * (sum(p for _, p in s) - 1) + 5 for s in seqs]
+    got = as_sets(shared_pages(table, held), table, held)
+    assert sorted(got) == list(range(6))
+    assert got[0] == [(0, 3, (0, 2, 3, 4, 5)), (3, 5, (0, 3)), (5, -1, (0,))]
+    assert got[5] == [(0, 3, (0, 2, 3, 4, 5)), (3, 4, (2, 4, 5)), (4, 6, (4, 5)), (6, -1, (5,))]
+    assert got[1] == [(0, -1, (1,))]
+    assert shared_pages(table, held).pages_saved == 4 * 3 + 2 + 2 * 1 + 2
+
+
+def test_only_full_pages_count_as_shared():
+    table, _ = tables([[("a", 2)], [("a", 2)]], 2)
+    assert shared_pages(table, [127, 127]).nodes == [(0, 2, 0, 1), (0, 1, 1, -1), (1, 1, 1, -1)]
+    assert shared_pages(table, [63, 128]) is None           # the first may still write to its only page
+    assert shared_pages(table, [64, 63]) is None
+    assert shared_pages(table[:1], [128]) is None
+    other, _ = tables([[(None, 2)], [(None, 2)]], 2)
+    assert shared_pages(other, [128, 128]) is None
+
+
+def test_places_that_are_not_held_share_nothing():
+    table = np.zeros((3, 4), dtype=np.int32)                # (they all name page 0)
+    table[0, 0], table[1, 0], table[2, 0] = 5, 6, 7
+    assert shared_pages(table, [70, 10, 90]) is None
+
+
+def test_chains_of_branches_end_at_a_depth():
+    n = MAX_LEVELS + 6                                      # every sequence leaves the chain a page later than the one before
+    seqs = [[("chain", i + 1), (None, 1)] for i in range(n)]
+    table, _ = tables(seqs, 3)
+    held = [64 * (i + 1) + 1 for i in range(n)]
+    got = as_sets(shared_pages(table, held), table, held)
+    assert max(len(nodes) for nodes in got.values()) == MAX_LEVELS + 1
+
+
+def random_step(rng):
+    branches, levels = int(rng.integers(1, 5)), int(rng.integers(1, 3))
+    common, seqs, held, news = int(rng.integers(0, 30)), [], [], []
+    for b in range(branches):
+        deep = int(rng.integers(1, 12))
+        for _ in range(int(rng.integers(1, 40))):
+            own = int(rng.integers(1, 9))
+            s = [("all", common)] + ([(b, deep)] if levels > 1 else []) + [(None, own)]
+            n = int(rng.integers(1, min(64 * own, 90) + 1)) if rng.random() < 0.3 else 1
+            seqs.append(s)
+            news.append(n)
+            held.append(64 * sum(p for _, p in s) - int(rng.integers(0, 64)) - n)
+            held[-1] = max(held[-1], 64 * sum(p for _, p in s[:-1]))
+    return tables(seqs, int(rng.integers(1 << 30)))[0], held, news
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_items_cover_what_every_row_sees_once(seed):
+    rng = np.random.default_rng(seed)
+    table, held, news = random_step(rng)
+    found = shared_pages(table, held)
+    if found is None:
+        return
+    starts = np.concatenate([[0], np.cumsum(news)])
+    context = [h + n for h, n in zip(held, news)]
+    for columns, group, nkv in ((128, 4, 8), (128, 1, 2), (128, 32, 1), (128, 7, 4), (16, 2, 4), (16, 16, 1), (16, 24, 2)):
+        items, order, part_start, parts, most = shared.plan(starts, context, found, group, nkv, columns, 512)
+        assert sorted(order.tolist()) == list(range(starts[-1]))
+        assert most == items[:, 1].max() and (most * group <= columns or (most == 1 and columns == 16))
+        pieces, owner = {}, {}
+        for row0, rows, seq, page, end, part0 in items[:, :6].tolist():
+            assert rows > 0 and end > page >= 0 and 0 <= row0 and row0 + rows <= len(order)
+            for r in range(rows):
+                token = int(order[row0 + r])
+                i = int(np.searchsorted(starts, token, side="right")) - 1
+                assert (table[i, page:end] == table[seq, page:end]).all() and end <= -(-context[i] // 64)
+                pieces.setdefault(token, []).append((page, end))
+                assert part0 + r not in owner
+                owner[part0 + r] = token
+        assert sorted(owner) == list(range(len(parts)))
+        for t, token in enumerate(order.tolist()):
+            assert [owner[p] for p in parts[part_start[t]:part_start[t + 1]]] == [token] * (part_start[t + 1] - part_start[t])
+            i = int(np.searchsorted(starts, token, side="right")) - 1
+            position, at = held[i] + token - starts[i], 0
+            for page, end in sorted(pieces[token]):
+                assert page == at
+                at = end
+            assert at >= position // 64 + 1
+
+
+def test_what_the_shared_attention_refuses():
+    kv = LayerKV(torch.zeros(4, 2, 64, 64), torch.zeros(4, 2, 64, 64), torch.zeros(2, 2, dtype=torch.int32), 64, 0)
+    meta = batch.pack([StepEntry(0, [0], [0]), StepEntry(1, [0], [0])], [64, 64], "cpu")
+    q = torch.zeros(2, 4 * 64)
+    with pytest.raises(BackendError, match="share no pages"):
+        shared.attention(q, meta, kv, q, 4, 2, 64, 0.125)
+    meta.shared = shared_pages(np.array([[1, 2], [1, 3]]), [64, 64])
+    with pytest.raises(BackendError, match="on the GPU"):
+        shared.attention(q, meta, kv, q, 4, 2, 64, 0.125)
+    for bad in ((3, 2, 64), (4, 2, 62), (4, 2, 260), (4, 0, 64)):
+        with pytest.raises(BackendError, match="refuses"):
+            shared.attention(q, meta, kv, q, *bad, 0.125)
+    windowed = LayerKV(kv.k, kv.v, kv.page_table, 64, 128)
+    keys_only = LayerKV(kv.k, None, kv.page_table, 64, 0)
+    for other in (windowed, keys_only, LayerKV(kv.k.bfloat16(), kv.v.bfloat16(), kv.page_table, 64, 0)):
+        with pytest.raises(BackendError, match="refuses"):
+            shared.attention(q, meta, other, q, 4, 2, 64, 0.125)
+
+
+def call(**changed):
+    args = dict(q=None, k=None, v=None, out=None, dtype=1, po=None, pml=None, items=None, n_items=1, max_rows=1, order=None, start=None,
+                parts=None, n_rows=1, positions=None, slots=None, table=None, max_pages=1, nq=4, nkv=2, hd=64, scale=0.1, softcap=0.0,
+                sinks=None, stream=None)
+    args.update(changed)
+    lib.call("attention_shared", "hb_attn_shared", *args.values())
+
+
+@pytest.mark.parametrize("changed, text", [
+    ({"nq": 5}, "do not group"), ({"n_rows": 0}, "empty"), ({"n_items": 0}, "empty"), ({"hd": 96}, "32, 64 or 128"), ({"dtype": 7}, "dtype"),
+    ({"max_rows": 65}, "exceed 128 columns"), ({"scale": 0.0}, "positive"), ({"softcap": -1.0}, "positive"),
+    ({"scale": float("nan")}, "positive"), ({"n_rows": 1 << 30}, "exceed|too many rows"), ({"n_items": 1 << 30}, "too many items"),
+    ({"dtype": 0, "hd": 62}, "whole quads"), ({"dtype": 0, "hd": 260}, "up to 256"), ({"dtype": 0, "k": 8}, "16-byte"),
+    ({"dtype": 0, "n_items": 1 << 30}, "too many items")])
+def test_calls_that_the_entry_refuses(changed, text):
+    with pytest.raises(BackendError, match=text):
+        call(**changed)
