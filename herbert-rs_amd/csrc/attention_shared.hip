@@ -17,221 +17,442 @@
 
 HB_MODULE_ERROR_SLOT()
 
-// What an item says, 8 numbers each: its first row in the order of the rows, how many (0: nothing here), the sequence whose
-// page table names its pages, its first page and the one behind its last, its first partial result.
+// What an item says, 8 numbers each: its first row in the order of the rows, how many (0: nothing here), the slot whose
+// page table names its pages, its first page and the one behind its last, where its rows' places among the partial results are
+// listed, whether there is a place in its pages that one of its rows does not see, and whether it stands for four items, a wave each,
+// that lie from its first number on.
 #define ITEM_INTS 8
 struct Item {
-    int row0, rows, seq, page0, page1, part0;
+    int row0, rows, slot, page0, page1, list0, masked, four;
     __device__ __forceinline__ explicit Item(const int* p)
-        : row0(p[0]), rows(p[1]), seq(p[2]), page0(p[3]), page1(p[4]), part0(p[5]) {}
+        : row0(p[0]), rows(p[1]), slot(p[2]), page0(p[3]), page1(p[4]), list0(p[5]), masked(p[6]), four(p[7]) {}
 };
 
 // ---------------------------------------------------------------- bfloat16
-// The values of a page that some column does not see whole, before their product: those of keys that no column sees are whatever lay
-// in the page and become zeros, since a weight of zero does not hide what is not finite. (va: rows d * 32 + c32, keys kb * 32 +
-// h2 * 16 + g2 * 8 + e.)
+// A workgroup is an item x a kv head, four waves. S^T = K Q^T and O^T = V^T P^T as in the other attention kernels.
+//
+// Wide items (more than 64 columns, every page seen whole): a wave is a tile of 32 columns, the pages go through a ring of LDS stages
+// once for all four, the next page's scores on the matrix cores while this one's exponentials are worked out.
+// Narrow ones: operands stream from memory into registers, half a page at a time, in 16 x 16 x 32 products, whose operands are 64
+// neighbouring bytes of a row; a wave has 16 or 32 columns, the waves of a tile (four, or two each of two tiles) take the pages
+// in turn and add up their results through LDS. Short ones of up to 32 columns are a wave each, four to a workgroup. With more than 64
+// columns (a sequence's own rows over the pages that they see in part) a wave is a tile of 32 here, too.
+// 256 registers and 66 KB of LDS: two workgroups a CU, so that items that wait for memory and items that compute overlap.
 template <int HD>
-__device__ __forceinline__ void hide_values(bf16x8 (&va)[HD / 32][2][2], int page0, int g2, int seen_last) {
-    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+struct SharedSizes {
+    static constexpr int STAGE = PAGE * HD;
+    static constexpr int RING = 4 * STAGE * 2;                                     // two stages of keys, two of values
+    static constexpr int SUMS = 4 * 2 * (HD / 16) * 64 * 16;                       // four waves' sums
+    static constexpr int HANDED = SUMS + 4 * 2 * 64 * 8;                           // and their references and denominators
+    static constexpr int LDS = RING > HANDED ? RING : HANDED;
+};
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ float max_of_rows(float v) {        // over the four lanes 16 apart
+    const unsigned u = __float_as_uint(v);
+    const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    return max_with_other_half(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+
+// What the kernel's two forms share.
+struct SharedArgs {
+    const bf16 *q, *k_cache, *v_cache;
+    float *partial_o, *partial_ml;
+    const int *order, *positions, *parts;
+    int nq, nkv, kvh, G;
+    float c, cap;
+};
+
+// A narrow item's wave: NT tiles of 16 columns from column col0 on, every phases-th page of the item from the phase-th on. With more than one
+// phase all waves of the workgroup come here (there is a barrier).
+// An operand of half a page: keys (row 4 g + i of block b: key 8 g + 4 b + i, so that a lane's scores are 8 neighbouring keys), g = lane / 16.
+template <int HD, int NT>
+__device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it, const int* pt, int cols, int col0, int phase, int phases,
+                                            int wave, int lane, char* lds) {
+    constexpr int STEPS = HD / 32, BLOCKS = HD / 16, STAGE = PAGE * HD;
+    constexpr int DEPTH = NT == 1 ? 2 : 1;               // halves of a page in flight
+    const int c16 = lane & 15, g = lane >> 4;
+    int token[NT], head[NT], place[NT], pos[NT];
+    bool mine[NT];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
+    for (int t = 0; t < NT; ++t) {
+        const int col = col0 + 16 * t + c16;
+        mine[t] = col < cols;
+        const int r = (mine[t] ? col : cols - 1) / A.G;
+        head[t] = A.kvh * A.G + (mine[t] ? col : cols - 1) % A.G;
+        token[t] = A.order[it.row0 + r];
+        place[t] = A.parts[it.list0 + r];
+        pos[t] = 0x7ffffffe;
+    }
+    bf16x8 ka[DEPTH][2][STEPS], va[DEPTH][BLOCKS], qreg[NT][STEPS];
+    const int k_lane = (8 * (c16 >> 2) + (c16 & 3)) * HD + g * 8, v_lane = c16 * PAGE + g * 8;
+    // (h: half of a page, 2 x its place among the item's pages + which)
+    auto load_keys = [&](int h, bf16x8 (&k)[2][STEPS]) {
+        const bf16* kp = A.k_cache + ((size_t)pt[it.page0 + (h >> 1)] * A.nkv + A.kvh) * STAGE + (h & 1) * 32 * HD + k_lane;
 #pragma unroll
-        for (int h2 = 0; h2 < 2; ++h2) {
-            const int seen = seen_last + 1 - (page0 + kb * 32 + h2 * 16 + g2 * 8);      // of the eight
-            u32x4 keep;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) keep[i] = seen >= 2 * i + 2 ? 0xffffffffu : seen == 2 * i + 1 ? 0xffffu : 0u;
+            for (int s = 0; s < STEPS; ++s) k[b][s] = *(const bf16x8*)(kp + b * 4 * HD + s * 32);
+    };
+    auto load_values = [&](int h, bf16x8 (&v)[BLOCKS]) {
+        const bf16* vp = A.v_cache + ((size_t)pt[it.page0 + (h >> 1)] * A.nkv + A.kvh) * STAGE + (h & 1) * 32 + v_lane;
 #pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
-                va[d][kb][h2] = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, va[d][kb][h2]) & keep);
+        for (int d = 0; d < BLOCKS; ++d) v[d] = *(const bf16x8*)(vp + d * 16 * PAGE);
+    };
+    const int halves = col0 < cols ? 2 * (it.page1 - it.page0) : 0;
+    auto next = [&](int h) { return (h & 1) ? h + 2 * phases - 1 : h + 1; };      // this wave's next half
+    int h = 2 * phase;
+    if (h < halves) {                                     // (a page is two halves: the second is there too)
+        load_keys(h, ka[0]);
+        load_values(h, va[0]);
+        if constexpr (DEPTH == 2) {
+            load_keys(h + 1, ka[1]);
+            load_values(h + 1, va[1]);
         }
-}
-
-// What is left of them that is not finite is taken out of the product as well and added here, one key after another, to the
-// columns that see it. (pb: this lane's weights of its column; a row of the output is entry d * 32 + 8 (i / 4) + 4 g2 + i % 4.)
-template <int HD>
-__device__ __forceinline__ void add_not_finite(bf16x8 (&va)[HD / 32][2][2], const bf16x8 (&pb)[2][2], f32x16 (&oacc)[HD / 32],
-                                               const bf16* values, int page0, int pos, int c32, int g2) {
-    bool any = false;
+    }
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+    for (int t = 0; t < NT; ++t) {
+        const bf16* qrow = A.q + ((size_t)token[t] * A.nq + head[t]) * HD + g * 8;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int s = 0; s < STEPS; ++s) qreg[t][s] = *(const bf16x8*)(qrow + s * 32);
+    }
+    int seen_last = 0x7ffffffe;
+    bool alike = true;                                    // all columns see the same keys
+    if (it.masked) {
+        int seen_first = 0x7ffffffe;
+        seen_last = -1;
 #pragma unroll
-            for (int h2 = 0; h2 < 2; ++h2)
+        for (int t = 0; t < NT; ++t) {
+            pos[t] = A.positions[token[t]];
+            seen_last = max(seen_last, pos[t]);
+            seen_first = min(seen_first, pos[t]);
+        }
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const bool finite = fabsf((float)va[d][kb][h2][e]) < INFINITY;
-                    any |= !finite;
-                    va[d][kb][h2][e] = finite ? va[d][kb][h2][e] : (__bf16)0.f;
-                }
-    if (__builtin_amdgcn_ballot_w64(any) == 0) return;
-#pragma unroll 1
-    for (int j = 0; j < PAGE; ++j) {
-        const int kb = j >> 5, h2 = (j >> 4) & 1, from = c32 + 32 * ((j >> 3) & 1), e = j & 7;
-        float w = 0.f;
+        for (int off = 1; off < 16; off <<= 1) {
+            seen_last = max(seen_last, __shfl_xor(seen_last, off, 64));
+            seen_first = min(seen_first, __shfl_xor(seen_first, off, 64));
+        }
+        alike = seen_first == seen_last;
+    }
+    f32x4 oacc[NT][BLOCKS];
+    float m[NT], l[NT];
 #pragma unroll
-        for (int x = 0; x < 32; ++x)
-            if (x == kb * 16 + h2 * 8 + e) w = (float)pb[x >> 4][(x >> 3) & 1][x & 7];
-        w = __shfl(w, from, 64);
-        if (page0 + j > pos) continue;
+    for (int t = 0; t < NT; ++t) {
+        m[t] = -INFINITY;
+        l[t] = 0.f;
 #pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
+        for (int d = 0; d < BLOCKS; ++d) oacc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    auto half = [&](bf16x8 (&k)[2][STEPS], bf16x8 (&v)[BLOCKS]) {
+        const int key0 = it.page0 * PAGE + h * 32;
+        const int following = DEPTH == 2 ? h + 2 * phases : next(h);     // the half whose operands take these registers next
+        f32x4 st[NT][2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float v = hb_to_float(values[(d * 32 + 8 * (i >> 2) + 4 * g2 + (i & 3)) * PAGE + j]);
-                if (!(fabsf(v) < INFINITY)) oacc[d][i] = fmaf(w, v, oacc[d][i]);
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                st[t][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < STEPS; ++s) st[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][s], qreg[t][s], st[t][b], 0, 0, 0);
             }
+        __builtin_amdgcn_sched_barrier(0);
+        if (following < halves) load_keys(following, k);
+        __builtin_amdgcn_sched_barrier(0);
+        bf16x8 pb[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float mx = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float x = st[t][i >> 2][i & 3];
+                if (A.cap != 0.f) x = A.cap - 2.0f * A.cap * __builtin_amdgcn_rcpf(1.0f + fast_exp2(x * (2.0f * 1.4426950408889634f / A.cap)));
+                x = key0 + 8 * g + i <= pos[t] ? x : -INFINITY;
+                st[t][i >> 2][i & 3] = x;
+                mx = fmaxf(mx, x);
+            }
+            mx = max_of_rows(mx);
+            float corr = 1.0f;                            // (the reference moves up lazily: see softmax_page)
+            if ((mx - m[t]) * A.c > RESCALE_LOG2 || m[t] == -INFINITY) {
+                const float m_new = (mx == -INFINITY) ? m[t] : mx;
+                corr = (m[t] == -INFINITY) ? 0.f : fast_exp2((m[t] - m_new) * A.c);
+                m[t] = m_new;
+            }
+            const float mc = (m[t] == -INFINITY) ? 0.f : m[t] * A.c;
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float p = fast_exp2(fmaf(st[t][i >> 2][i & 3], A.c, -mc));
+                sum += p;
+                pb[t][i] = (__bf16)p;
+            }
+            l[t] = l[t] * corr + sum;
+            if (__builtin_amdgcn_ballot_w64(corr != 1.0f) != 0)
+#pragma unroll
+                for (int d = 0; d < BLOCKS; ++d) oacc[t][d] *= corr;
+        }
+        // Values of keys that no column sees are whatever lay in the page and become zeros: a weight of zero does not hide what
+        // is not finite. (The registers of the values themselves stay as they are: changed under a condition within this loop, the
+        // compiler took some of them for temporaries.)
+        const int seen = seen_last + 1 - (key0 + 8 * g);                 // of this lane's eight
+        u32x4 keep;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) keep[i] = seen >= 2 * i + 2 ? 0xffffffffu : seen == 2 * i + 1 ? 0xffffu : 0u;
+        uint32_t odd = 0;              // (an exponent of ones: its lowest bit added carries into the sign's place; two numbers a word)
+        if (!alike)
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    odd |= (((__builtin_bit_cast(u32x4, v[d])[i] & keep[i]) & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+        if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) {
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) {
+                const bf16x8 clean = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, v[d]) & keep);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, pb[t], oacc[t][d], 0, 0, 0);
+            }
+        } else {
+            // What is left that is not finite is taken out of the product, and the columns that see it get what their sums would
+            // be: a second product counts, for every entry and column, the keys whose value is +inf (1 each), -inf (128) or NaN
+            // (16384; of 32 keys no count runs into the next).
+            bf16x8 sees[NT];
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) sees[t][e] = key0 + 8 * g + e <= pos[t] ? (__bf16)1.f : (__bf16)0.f;
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) {
+                u32x4 x = __builtin_bit_cast(u32x4, v[d]) & keep, kind;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t ones = (((x[i] & 0x7f807f80u) + 0x00800080u) >> 15) & 0x00010001u;
+                    const uint32_t nan = ones & (((x[i] & 0x007f007fu) + 0x007f007fu) >> 7);
+                    const uint32_t minus = ones & ~nan & (x[i] >> 15), plus = ones & ~nan & ~minus;
+                    kind[i] = nan * 0x4680u | minus * 0x4300u | plus * 0x3f80u;      // 16384, 128, 1
+                    x[i] &= ~(ones * 0xffffu);
+                }
+                const bf16x8 clean = __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const f32x4 counts = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kind), sees[t],
+                                                                                 f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+                    oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, pb[t], oacc[t][d], 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int n = (int)counts[i];
+                        const bool plus = n & 127, minus = n & 0x3f80;
+                        oacc[t][d][i] += n >= 16384 || (plus && minus) ? __uint_as_float(0x7fc00000u) : plus ? INFINITY : minus ? -INFINITY : 0.f;
+                    }
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if (following < halves) load_values(following, v);
+        __builtin_amdgcn_sched_barrier(0);
+        h = next(h);
+    };
+    while (h < halves) {
+        half(ka[0], va[0]);
+        if constexpr (DEPTH == 2) half(ka[1], va[1]);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        l[t] += __shfl_xor(l[t], 16, 64);
+        l[t] += __shfl_xor(l[t], 32, 64);
+    }
+    auto leave = [&](int t, int d) {
+        if (mine[t]) *(f32x4*)(A.partial_o + ((size_t)place[t] * A.nq + head[t]) * HD + d * 16 + 4 * g) = oacc[t][d];
+    };
+    auto leave_ml = [&](int t, float top, float total) {
+        if (mine[t] && g == 0) ((float2*)A.partial_ml)[(size_t)place[t] * A.nq + head[t]] = make_float2(top, total);
+    };
+    // the waves of a tile add up what they have: each the blocks that are its own (the x-th: phase x % PHASES)
+    auto join = [&](auto phases_tag) {
+        constexpr int PHASES = decltype(phases_tag)::value, TILES = 4 / PHASES;
+        f32x4* const sums = (f32x4*)lds;                                 // [wave][tile and block][lane]
+        float2* const ml = (float2*)(lds + SharedSizes<HD>::SUMS);       // [wave][tile][lane]
+        const int tile = wave % TILES;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            ml[(wave * NT + t) * 64 + lane] = make_float2(m[t], l[t]);
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d)
+                if ((t * BLOCKS + d) % PHASES != phase) sums[((wave * NT + t) * BLOCKS + d) * 64 + lane] = oacc[t][d];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float2 other[PHASES];
+            float top = -INFINITY, total = 0.f;
+#pragma unroll
+            for (int f = 0; f < PHASES; ++f) {
+                other[f] = ml[((f * TILES + tile) * NT + t) * 64 + lane];
+                top = fmaxf(top, other[f].x);
+            }
+#pragma unroll
+            for (int f = 0; f < PHASES; ++f) {
+                other[f].x = other[f].x == -INFINITY ? 0.f : fast_exp2((other[f].x - top) * A.c);
+                total = fmaf(other[f].x, other[f].y, total);
+            }
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) {
+                if ((t * BLOCKS + d) % PHASES != phase) continue;
+                f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int f = 0; f < PHASES; ++f) {
+                    f32x4 x = oacc[t][d];
+                    if (f != phase) x = sums[(((f * TILES + tile) * NT + t) * BLOCKS + d) * 64 + lane];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[e] = fmaf(other[f].x, x[e], o[e]);
+                }
+                oacc[t][d] = o;
+                leave(t, d);
+            }
+            if (phase == 0) leave_ml(t, top, total);
+        }
+    };
+    if (phases == 4) {
+        join(std::integral_constant<int, 4>{});
+    } else if (NT == 2 && phases == 2) {
+        join(std::integral_constant<int, 2>{});
+    } else {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            leave_ml(t, m[t], l[t]);
+#pragma unroll
+            for (int d = 0; d < BLOCKS; ++d) leave(t, d);
+        }
     }
 }
 
-// A workgroup: an item x a kv head. Its four waves are as many tiles of 32 columns as the item fills (1, 2 or 4); where those are
-// fewer than four the waves of a tile take the pages in turn and add up their results through LDS.
-// S^T = K Q^T and O^T = V^T P^T as in the decode kernel: operands stream from memory into registers, P stays there.
+// A wide item's wave: 32 columns from column col0 on (active: some of them exist). All four waves come here.
 template <int HD>
-__global__ void __launch_bounds__(256)
-attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache,
-                   float* __restrict__ partial_o, float* __restrict__ partial_ml, const int* __restrict__ items,
-                   const int* __restrict__ order, const int* __restrict__ positions, const int* __restrict__ slots,
-                   const int* __restrict__ page_table, int max_pages, int nq, int nkv, float c, float cap) {
-    constexpr int HANDED = (HD / 2 + 2) * 64;                     // floats that a wave hands over
-    extern __shared__ __attribute__((aligned(16))) float handed[];   // [3][HANDED]
-    const int kvh = blockIdx.x % nkv;
-    const Item it(items + (size_t)(blockIdx.x / nkv) * ITEM_INTS);
-    if (it.rows == 0) return;
-    const int G = nq / nkv, cols = it.rows * G;
-    const int tiles = cols <= 32 ? 1 : cols <= 64 ? 2 : 4, phases = 4 / tiles;
-    const int lane = threadIdx.x & 63, c32 = lane & 31, g2 = lane >> 5;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int tile = wave % tiles, phase = wave / tiles;
-    const int col = tile * 32 + c32;
-    const bool mine = col < cols;
-    const int r = (mine ? col : cols - 1) / G, head = kvh * G + (mine ? col : cols - 1) % G;
-    const int token = order[it.row0 + r];
-    const int pos = positions[token];
-    int seen_last = pos, seen_first = pos;                        // the last key that some, and that every column sees
+__device__ __forceinline__ void wide_item(const SharedArgs& A, const Item& it, const int* pt, int cols, int wave, int lane, bf16* lds) {
+    constexpr int BLOCKS = HD / 32, STAGE = PAGE * HD;
+    constexpr int KCH = HD / 8, KRPB = 128 / HD > 0 ? 128 / HD : 1, KROWS = 512 / HD, LOADS = HD / 32;
+    const int c32 = lane & 31, g2 = lane >> 5, krow = perm(c32);
+    bf16* const Ks = lds;
+    bf16* const Vs = Ks + 2 * STAGE;
+    const int n = it.page1 - it.page0;
+    const bool active = wave * 32 < cols;
+    int k_off[LOADS], v_off[LOADS];
 #pragma unroll
-    for (int off = 1; off < 32; off <<= 1) {
-        seen_last = max(seen_last, __shfl_xor(seen_last, off, 64));
-        seen_first = min(seen_first, __shfl_xor(seen_first, off, 64));
+    for (int i = 0; i < LOADS; ++i) {
+        const int instr = wave * LOADS + i;
+        const int kr = instr * KROWS + lane / KCH;
+        k_off[i] = kr * HD + (((lane % KCH) ^ ((kr / KRPB) % KCH)) * 8);
+        const int vr = instr * 8 + lane / 8;
+        v_off[i] = vr * PAGE + (((lane & 7) ^ ((vr >> 1) & 7)) * 8);
     }
-    const int* pt = page_table + (size_t)slots[it.seq] * max_pages;
-    const int page_end = tile * 32 < cols ? min(it.page1, seen_last / PAGE + 1) : 0;
-
+    auto issue_keys = [&](int i, int stage) {
+        const bf16* kp = A.k_cache + ((size_t)pt[it.page0 + i] * A.nkv + A.kvh) * STAGE;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) hb_load_to_lds(kp + k_off[j], Ks + stage * STAGE + (wave * LOADS + j) * 512);
+    };
+    auto issue_values = [&](int i, int stage) {
+        const bf16* vp = A.v_cache + ((size_t)pt[it.page0 + i] * A.nkv + A.kvh) * STAGE;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) hb_load_to_lds(vp + v_off[j], Vs + stage * STAGE + (wave * LOADS + j) * 512);
+    };
+    issue_keys(0, 0);
+    issue_values(0, 0);
+    if (n > 1) issue_keys(1, 1);
+    const int col = wave * 32 + c32;
+    const bool mine = col < cols;
+    const int r = (mine ? col : cols - 1) / A.G, head = A.kvh * A.G + (mine ? col : cols - 1) % A.G;
+    const int token = A.order[it.row0 + r], place = A.parts[it.list0 + r];
     bf16x8 qreg[HD / 16];
     {
-        const bf16* qrow = q + ((size_t)token * nq + head) * HD + g2 * (HD / 2);
+        const bf16* qrow = A.q + ((size_t)token * A.nq + head) * HD + g2 * 8;
 #pragma unroll
-        for (int s = 0; s < HD / 16; ++s) qreg[s] = *(const bf16x8*)(qrow + s * 8);
+        for (int s = 0; s < HD / 16; ++s) qreg[s] = *(const bf16x8*)(qrow + s * 16);
     }
-    f32x16 oacc[HD / 32];
+    f32x16 oacc[BLOCKS];
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+    for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i) oacc[d][i] = 0.f;
     float m = -INFINITY, l = 0.f;
-    const int krow = perm(c32);
-    bf16x8 ka[2][HD / 16];
-    bf16x8 va[HD / 32][2][2];
-    auto load_keys = [&](int p) {
-        const bf16* kp = k_cache + ((size_t)pt[p] * nkv + kvh) * PAGE * HD + g2 * (HD / 2);
+    PrefillLane ln;
+    ln.c32 = c32;
+    ln.g2 = g2;
+    ln.krow = krow;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) ln.k_read[kb] = ((kb * 32 + krow) / KRPB) % KCH;
+    ln.v_swz = (c32 >> 1) & 7;
+    auto step = [&](auto parity_tag, int i, f32x16 (&st)[2], f32x16 (&nxt)[2]) {
+        // landed, for every wave after the barrier: the values of this page and the keys of the next; and
+        // nobody reads any more the stages that the next loads fill
+        hb_wait_vmcnt<0>();
+        hb_workgroup_barrier();
+        if (i + 2 < n) issue_keys(i + 2, i & 1);
+        if (i + 1 < n) issue_values(i + 1, (i + 1) & 1);
+        if (!active) return;
+        float corr;
+        if (A.cap != 0.f) cap_scores(st, A.cap);
+        const float mc = softmax_reference<false>(st, g2, 0, 0, 0, A.c, m, corr);
+        rescale(oacc, corr);
+        constexpr int PAR = decltype(parity_tag)::value;
+        prefill_step_products<HD>(Ks + ((PAR + 1) & 1) * STAGE, Vs + PAR * STAGE, st, nxt, oacc, qreg, ln, A.c, mc, corr, l);
+    };
+    hb_wait_vmcnt<0>();
+    hb_workgroup_barrier();
+    f32x16 sa[2], sb[2];
+    if (active) {
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-            for (int s = 0; s < HD / 16; ++s) ka[kb][s] = *(const bf16x8*)(kp + (kb * 32 + krow) * HD + s * 8);
-    };
-    auto load_values = [&](int p) {
-        const bf16* vp = v_cache + ((size_t)pt[p] * nkv + kvh) * HD * PAGE + g2 * 8;
+            for (int i = 0; i < 16; ++i) sa[kb][i] = 0.f;
 #pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
+        for (int s = 0; s < HD / 16; ++s)
 #pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int h2 = 0; h2 < 2; ++h2) va[d][kb][h2] = *(const bf16x8*)(vp + (d * 32 + c32) * PAGE + kb * 32 + h2 * 16);
-    };
-    int p = it.page0 + phase;
-    if (p < page_end) {
-        load_keys(p);
-        load_values(p);
+            for (int kb = 0; kb < 2; ++kb) {
+                const bf16x8 ka = *(const bf16x8*)(Ks + (kb * 32 + krow) * HD + (((2 * s + g2) ^ ln.k_read[kb]) * 8));
+                sa[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, qreg[s], sa[kb], 0, 0, 0);
+            }
     }
-    for (; p < page_end; p += phases) {
-        f32x16 st[2];
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) st[kb][i] = 0.f;
-#pragma unroll
-            for (int s = 0; s < HD / 16; ++s)
-                st[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka[kb][s], qreg[s], st[kb], 0, 0, 0);
-        }
-        if (p + phases < page_end) load_keys(p + phases);
-        float corr;
-        bf16x8 pb[2][2];
-        if (cap != 0.f) cap_scores(st, cap);
-        const int page0 = p * PAGE;
-        if (page0 + PAGE - 1 <= seen_first) {
-            softmax_page<false>(st, g2, page0, 0, pos, c, m, l, corr, pb);
-        } else {
-            softmax_page<true>(st, g2, page0, 0, pos, c, m, l, corr, pb);
-            hide_values<HD>(va, page0, g2, seen_last);
-        }
-        rescale(oacc, corr);
-        if (page0 + PAGE - 1 > seen_first && seen_first != seen_last)
-            add_not_finite<HD>(va, pb, oacc, v_cache + ((size_t)pt[p] * nkv + kvh) * HD * PAGE, page0, pos, c32, g2);
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-                for (int h2 = 0; h2 < 2; ++h2)
-                    oacc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(va[d][kb][h2], pb[kb][h2], oacc[d], 0, 0, 0);
-        if (p + phases < page_end) load_values(p + phases);
+    for (int i = 0; i < n; i += 2) {
+        step(std::integral_constant<int, 0>{}, i, sa, sb);
+        if (i + 1 < n) step(std::integral_constant<int, 1>{}, i + 1, sb, sa);
     }
     l += __shfl_xor(l, 32, 64);
-    if (phases > 1) {
-        if (phase > 0) {
-            float* const hand = handed + (wave - tiles) * HANDED + lane;
-            hand[0] = m;
-            hand[64] = l;
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) hand[(2 + d * 16 + i) * 64] = oacc[d][i];
-        }
-        __syncthreads();
-        if (phase > 0) return;
-        float top = m;
-        for (int f = 1; f < phases; ++f) top = fmaxf(top, handed[((f - 1) * tiles + tile) * HANDED + lane]);
-        const float own = m == -INFINITY ? 0.f : fast_exp2((m - top) * c);
-        l *= own;
-#pragma unroll
-        for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) oacc[d][i] *= own;
-        for (int f = 1; f < phases; ++f) {
-            const float* const hand = handed + ((f - 1) * tiles + tile) * HANDED + lane;
-            const float share = hand[0] == -INFINITY ? 0.f : fast_exp2((hand[0] - top) * c);
-            l = fmaf(share, hand[64], l);
-#pragma unroll
-            for (int d = 0; d < HD / 32; ++d)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) oacc[d][i] = fmaf(share, hand[(2 + d * 16 + i) * 64], oacc[d][i]);
-        }
-        m = top;
-    }
     if (!mine) return;
-    const size_t part = (size_t)(it.part0 + r) * nq + head;
-    if (g2 == 0) {
-        partial_ml[part * 2] = m;
-        partial_ml[part * 2 + 1] = l;
-    }
-    float* const po = partial_o + part * HD;
+    const size_t part = (size_t)place * A.nq + head;
+    if (g2 == 0) ((float2*)A.partial_ml)[part] = make_float2(m, l);
+    float* const po = A.partial_o + part * HD;
 #pragma unroll
-    for (int d = 0; d < HD / 32; ++d)
+    for (int d = 0; d < BLOCKS; ++d)
 #pragma unroll
         for (int qd = 0; qd < 4; ++qd)
-            *(f32x4*)(po + d * 32 + 8 * qd + 4 * g2) =
-                f32x4{oacc[d][4 * qd], oacc[d][4 * qd + 1], oacc[d][4 * qd + 2], oacc[d][4 * qd + 3]};
+            *(f32x4*)(po + d * 32 + 8 * qd + 4 * g2) = f32x4{oacc[d][4 * qd], oacc[d][4 * qd + 1], oacc[d][4 * qd + 2], oacc[d][4 * qd + 3]};
+}
+
+template <int HD>
+__global__ void __launch_bounds__(256, 2)
+attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache,
+                   float* __restrict__ partial_o, float* __restrict__ partial_ml, const int* __restrict__ items,
+                   const int* __restrict__ order, const int* __restrict__ parts, const int* __restrict__ positions,
+                   const int* __restrict__ page_table, int max_pages, int nq, int nkv, float c, float cap) {
+    // (of the launch, not of the kernel: see the prompt kernels)
+    extern __shared__ __attribute__((aligned(1024))) char shared_lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    Item it(items + (size_t)(blockIdx.x / nkv) * ITEM_INTS);
+    const bool four = it.four;
+    if (four) it = Item(items + (size_t)(it.row0 + wave) * ITEM_INTS);
+    if (it.rows == 0) return;
+    const SharedArgs A = {q, k_cache, v_cache, partial_o, partial_ml, order, positions, parts, nq, nkv, (int)(blockIdx.x % nkv), nq / nkv, c, cap};
+    const int cols = it.rows * A.G;
+    const int* pt = page_table + (size_t)it.slot * max_pages;
+    if (cols > 64 && !it.masked) {
+        wide_item<HD>(A, it, pt, cols, wave, lane, (bf16*)shared_lds);
+        return;
+    }
+    const int tiles = cols <= 32 ? 1 : cols <= 64 ? 2 : 4, phases = four ? 1 : 4 / tiles;
+    const int tile = four ? 0 : wave % tiles, phase = four ? 0 : wave / tiles;
+    if (cols <= 16) narrow_item<HD, 1>(A, it, pt, cols, 0, phase, phases, wave, lane, shared_lds);
+    else narrow_item<HD, 2>(A, it, pt, cols, tile * 32, phase, phases, wave, lane, shared_lds);
 }
 
 // ---------------------------------------------------------------- float32
@@ -242,7 +463,7 @@ template <int NB>
 __global__ void __launch_bounds__(256)
 attn_shared_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_cache, const float* __restrict__ v_cache,
                        float* __restrict__ partial_o, float* __restrict__ partial_ml, const int* __restrict__ items,
-                       const int* __restrict__ order, const int* __restrict__ positions, const int* __restrict__ slots,
+                       const int* __restrict__ order, const int* __restrict__ parts, const int* __restrict__ positions,
                        const int* __restrict__ page_table, int max_pages, int nq, int nkv, int hd, float scale, float softcap,
                        int col_tiles) {
     constexpr int DB = 4 * NB, QLD = 16 * DB + 4, SLD = PAGE + 4;
@@ -255,24 +476,29 @@ attn_shared_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_
     if (col0 >= cols) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int r = lane & 15, g4 = lane >> 4;
-    // the queries, zeros beyond the head's entries and in columns that are nobody's, every 16 entries transposed
-    for (int i = tid; i < 16 * 16 * DB; i += 256) {
-        const int cl = col0 + i / (16 * DB), d = i % (16 * DB);
-        float v = 0.f;
-        if (cl < cols && d < hd) v = q[((size_t)order[it.row0 + cl / G] * nq + kvh * G + cl % G) * hd + d];
-        qs[(i / (16 * DB)) * QLD + (d & ~15) + 4 * (d & 3) + ((d >> 2) & 3)] = v;
-    }
+    const int* pt = page_table + (size_t)it.slot * max_pages;
     const int col = col0 + r;
     const bool mine = col < cols;
     const int row = (mine ? col : cols - 1) / G, head = kvh * G + (mine ? col : cols - 1) % G;
-    const int pos = positions[order[it.row0 + row]];
+    const int pos = positions[order[it.row0 + row]], place = parts[it.list0 + row];
+    // the queries, zeros beyond the head's entries and in columns that are nobody's, every 16 entries transposed: 16 threads a column
+    {
+        const int mc = tid >> 4, cl = col0 + mc;
+        const float* src = q + ((size_t)order[it.row0 + (cl < cols ? cl : cols - 1) / G] * nq + kvh * G + (cl < cols ? cl : cols - 1) % G) * hd;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int d = 4 * ((tid & 15) + 16 * i);
+            const f32x4 v = d < hd && cl < cols ? *(const f32x4*)(src + d) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) qs[mc * QLD + (d & ~15) + 4 * e + ((d >> 2) & 3)] = v[e];
+        }
+    }
     int seen_last = pos, seen_first = pos;
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) {
         seen_last = max(seen_last, __shfl_xor(seen_last, off, 64));
         seen_first = min(seen_first, __shfl_xor(seen_first, off, 64));
     }
-    const int* pt = page_table + (size_t)slots[it.seq] * max_pages;
     const int page_end = min(it.page1, seen_last / PAGE + 1);
     f32x4 acc[NB];
 #pragma unroll
@@ -299,19 +525,24 @@ attn_shared_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_
     }
     __syncthreads();
     for (int p = it.page0; p < page_end; ++p) {
-        const int page0 = p * PAGE, next = p + 1 < page_end ? p + 1 : p;
+        const int page0 = p * PAGE;
+        const bool more = p + 1 < page_end;
         if (hd < 16 * DB)
 #pragma unroll
             for (int b = 0; b < DB; ++b) key[b] = 16 * b + 4 * g4 < hd ? key[b] : f32x4{0.f, 0.f, 0.f, 0.f};
-        f32x4 dots = {0.f, 0.f, 0.f, 0.f};
+        // (four chains side by side: a quarter of the roundings one after the other, and none waits for another)
+        f32x4 chain[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) chain[i] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int b = 0; b < DB; ++b) {
             transpose_quads(key[b]);
             const f32x4 qq = *(const f32x4*)&qs[r * QLD + 16 * b + 4 * g4];
 #pragma unroll
-            for (int s = 0; s < 4; ++s) dots = mfma_k4(key[b][s], qq[s], dots);
+            for (int s = 0; s < 4; ++s) chain[b & 3] = mfma_k4(key[b][s], qq[s], chain[b & 3]);
         }
-        load_keys(next);
+        f32x4 dots = (chain[0] + chain[1]) + (chain[2] + chain[3]);
+        if (more) load_keys(p + 1);
         dots *= scale;
         if (softcap > 0.f)
 #pragma unroll
@@ -376,18 +607,20 @@ attn_shared_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_
                         if (d0 + 4 * g4 + e < hd) acc[i][e] = fmaf(mine_w, at[(d0 + 4 * g4 + e) * PAGE + j], acc[i][e]);
                 }
             } else {
+                f32x4 half[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};     // (of the page)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     transpose_quads(v[b]);
 #pragma unroll
-                    for (int s = 0; s < 4; ++s) acc[i] = mfma_k4(v[b][s], w[b][s], acc[i]);
+                    for (int s = 0; s < 4; ++s) half[b & 1] = mfma_k4(v[b][s], w[b][s], half[b & 1]);
                 }
+                acc[i] += half[0] + half[1];
             }
         }
-        load_values(next);
+        if (more) load_values(p + 1);
     }
     if (!mine) return;
-    const size_t part = (size_t)(it.part0 + row) * nq + head;
+    const size_t part = (size_t)place * nq + head;
     if (wave == 0 && g4 == 0) {
         partial_ml[part * 2] = m;
         partial_ml[part * 2 + 1] = l;
@@ -402,67 +635,82 @@ attn_shared_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_
 }
 
 // ---------------------------------------------------------------- joining
-// A wave a (token, query head): the partial results parts[part_start[t] ..] of the t-th row, in their order. T: the type that
-// leaves; c: what a difference of references is multiplied by for a power of two (float32: natural units, expf).
+// A wave a (token, query head): the partial results part_start[t] .. part_start[t + 1] - 1 of the t-th row, in their order. T: the type that
+// leaves; c: what a difference of references is multiplied by for a power of two (float32: natural units, expf). A chain of three waits:
+// where they lie, the results with their references, and the store.
 template <class T, int E>
 __global__ void __launch_bounds__(256)
 attn_shared_join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, T* __restrict__ out,
-                        const int* __restrict__ order, const int* __restrict__ part_start, const int* __restrict__ parts,
-                        int n_rows, int nq, int hd, float c, const float* __restrict__ sinks) {
+                        const int* __restrict__ order, const int* __restrict__ part_start, int n_rows, int nq, int hd, float c,
+                        const float* __restrict__ sinks) {
     constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int AHEAD = 8;
     const int lane = threadIdx.x & 63;
     const int at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int t = at / nq, h = at % nq;
     if (t >= n_rows) return;
-    const int first = part_start[t], n = part_start[t + 1] - first;
+    const int first = part_start[t], n = part_start[t + 1] - first, row = order[t];
+    const float* const po = partial_o + ((size_t)first * nq + h) * hd + E * lane;
+    const float2* const ml = (const float2*)partial_ml + (size_t)first * nq + h;
+    const size_t stride = (size_t)nq * hd;
+    const bool there = E * lane < hd;
+    float v[AHEAD][E];
+    auto ask = [&](int s) {                               // (places beyond the last: the last, with a weight of 0)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const float* p = po + (size_t)(s + u < n ? s + u : n - 1) * stride;
+#pragma unroll
+            for (int e = 0; e < E; ++e) v[u][e] = there ? p[e] : 0.f;
+        }
+    };
+    ask(0);
     auto weight = [&](float m, float top) { return m == -INFINITY ? 0.f : EXACT ? expf(m - top) : fast_exp2((m - top) * c); };
     float top = -INFINITY;
-    for (int s = lane; s < n; s += 64) top = fmaxf(top, partial_ml[((size_t)parts[first + s] * nq + h) * 2]);
+    float2 kept = make_float2(-INFINITY, 0.f);            // this lane's, of the first 64
+    for (int s = lane; s < n; s += 64) {
+        const float2 x = ml[(size_t)s * nq];
+        if (s == lane) kept = x;
+        top = fmaxf(top, x.x);
+    }
     top = hb_wave_max(top);
     float acc[E], total = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.f;
     for (int s0 = 0; s0 < n; s0 += 64) {
-        int part = 0;
-        float w = 0.f, term = 0.f;
-        if (s0 + lane < n) {
-            part = parts[first + s0 + lane];
-            const float2 ml = ((const float2*)partial_ml)[(size_t)part * nq + h];
-            w = weight(ml.x, top);
-            term = w * ml.y;
-        }
-        total += hb_wave_sum(term);
+        if (s0 > 0) kept = s0 + lane < n ? ml[(size_t)(s0 + lane) * nq] : make_float2(-INFINITY, 0.f);
+        const float w = weight(kept.x, top);
+        total += hb_wave_sum(w * kept.y);
         const int here = n - s0 < 64 ? n - s0 : 64;
-        for (int s = 0; s < here; ++s) {
-            const float ws = __shfl(w, s, 64);
-            const float* po = partial_o + ((size_t)__shfl(part, s, 64) * nq + h) * hd;
+        for (int s = 0; s < here; s += AHEAD) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int d = E * lane + e;
-                if (d < hd) acc[e] = fmaf(ws, po[d], acc[e]);
+            for (int u = 0; u < AHEAD; ++u) {
+                const float ws = __shfl(w, s + u < here ? s + u : 0, 64);
+#pragma unroll
+                for (int e = 0; e < E; ++e) acc[e] = s + u >= here || ws == 0.f ? acc[e] : fmaf(ws, v[u][e], acc[e]);
             }
+            if (s0 + s + AHEAD < n) ask(s0 + s + AHEAD);
         }
     }
     if (sinks) total += EXACT ? expf(sinks[h] - (top == -INFINITY ? 0.f : top)) : sink_share(sinks[h], top, c);
     const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
-    T* const dst = out + ((size_t)order[t] * nq + h) * hd;
+    if (!there) return;
+    T* const dst = out + ((size_t)row * nq + h) * hd + E * lane;
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        const int d = E * lane + e;
-        if (d < hd) dst[d] = hb_from_float<T>(acc[e] * inv);
-    }
+    for (int e = 0; e < E; ++e) dst[e] = hb_from_float<T>(acc[e] * inv);
 }
 
-// q, out [T, nq hd]; keys [pages, nkv, 64, hd], values [pages, nkv, hd, 64]; one storage type. items [n_items, 8]; order [n_rows],
-// part_start [n_rows + 1], parts [...]; partial_o [partial results, nq, hd], partial_ml [partial results, nq, 2]. max_rows: the most
-// rows of an item. softcap 0: none; sinks [nq] or null.
+// q, out [T, nq hd]; keys [pages, nkv, 64, hd], values [pages, nkv, hd, 64]; one storage type. items [n_items, 8] (and behind them those of
+// single waves); order [n_rows]; part_start [n_rows + 1]: where a row's partial results begin; parts: the places of the items' rows among
+// them; partial_o [partial results, nq, hd], partial_ml [partial results, nq, 2]. max_rows: the most rows of an item. softcap 0: none; sinks [nq] or null.
 extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, float* partial_o,
                               float* partial_ml, const int* items, int n_items, int max_rows, const int* order,
-                              const int* part_start, const int* parts, int n_rows, const int* positions, const int* slots,
+                              const int* part_start, const int* parts, int n_rows, const int* positions,
                               const int* page_table, int max_pages, int nq, int nkv, int hd, float scale, float softcap,
                               const float* sinks, hipStream_t stream) {
     HB_REQUIRE(n_rows > 0 && n_items > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "shared attention: empty input, or heads that do not group");
     HB_REQUIRE(scale > 0.f && softcap >= 0.f, "shared attention: the scale must be positive, a cap of the scores too");
+    HB_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)partial_o) % 16 == 0,
+               "shared attention: queries and pages lie on 16-byte borders");
     const int G = nq / nkv;
     const long long rows_of_heads = (long long)n_rows * nq;
     HB_REQUIRE(rows_of_heads <= 0x7fffffffLL - 4, "shared attention: too many rows for the grid");
@@ -475,13 +723,16 @@ extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_
         const dim3 grid((unsigned)(n_items * nkv));
 #define HB_SHARED(HD, E)                                                                                                     \
         {                                                                                                                    \
-            constexpr int lds = 3 * (HD / 2 + 2) * 64 * 4;                                                                   \
+            constexpr int lds = SharedSizes<HD>::LDS;                                                                        \
+            static const hipError_t allowed =                                                                                \
+                hipFuncSetAttribute((const void*)attn_shared_kernel<HD>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);   \
+            HB_REQUIRE(allowed == hipSuccess, "shared attention: %d bytes of LDS refused: %s", lds, hipGetErrorString(allowed)); \
             attn_shared_kernel<HD><<<grid, 256, lds, stream>>>((const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache,   \
-                                                               partial_o, partial_ml, items, order, positions, slots,        \
+                                                               partial_o, partial_ml, items, order, parts, positions,        \
                                                                page_table, max_pages, nq, nkv, c, cap);                      \
             HB_CHECK_LAUNCH("shared attention");                                                                             \
             attn_shared_join_kernel<bf16, E><<<join, 256, 0, stream>>>(partial_o, partial_ml, (bf16*)out, order, part_start, \
-                                                                       parts, n_rows, nq, hd, c, sinks);                     \
+                                                                       n_rows, nq, hd, c, sinks);                            \
         }
         if (hd == 32) HB_SHARED(32, 1)
         else if (hd == 64) HB_SHARED(64, 1)
@@ -489,19 +740,18 @@ extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_
 #undef HB_SHARED
     } else if (dtype == HB_F32) {
         HB_REQUIRE(hd > 0 && hd <= 256 && hd % 4 == 0, "shared attention: float32 heads of up to 256 entries in whole quads, not %d", hd);
-        HB_REQUIRE(((uintptr_t)k_cache | (uintptr_t)v_cache) % 16 == 0, "shared attention: pages on 16-byte borders");
         const long long col_tiles = ((long long)max_rows * G + 15) / 16;
         HB_REQUIRE((long long)n_items * nkv * col_tiles <= 0x7fffffffLL, "shared attention: too many items for the grid");
         const dim3 grid((unsigned)(n_items * nkv * col_tiles));
 #define HB_SHARED(NB, E)                                                                                                       \
         {                                                                                                                      \
             attn_shared_f32_kernel<NB><<<grid, 256, 0, stream>>>((const float*)q, (const float*)k_cache, (const float*)v_cache, \
-                                                                 partial_o, partial_ml, items, order, positions, slots,        \
+                                                                 partial_o, partial_ml, items, order, parts, positions,        \
                                                                  page_table, max_pages, nq, nkv, hd, scale, softcap,           \
                                                                  (int)col_tiles);                                              \
             HB_CHECK_LAUNCH("shared attention");                                                                               \
             attn_shared_join_kernel<float, E><<<join, 256, 0, stream>>>(partial_o, partial_ml, (float*)out, order, part_start, \
-                                                                        parts, n_rows, nq, hd, 0.f, sinks);                    \
+                                                                        n_rows, nq, hd, 0.f, sinks);                    \
         }
         if (hd <= 64) HB_SHARED(1, 1)
         else if (hd <= 128) HB_SHARED(2, 2)

@@ -44,6 +44,7 @@ class BatchMeta:
     unequal: int = 0           # how unequal the contexts' lengths are: 0 (alike), 1, 2 (see unequal_level)
     num_real: int = 0          # sequences that are no padding rows (0: all of them)
     static: object = None      # the StaticDecodeMeta whose buffers these are, if any
+    host_slots: np.ndarray = None   # the slots on the host
     shared: object = None      # the pages that sequences of this step hold together (cache.SharedPages); None: none
 
     def ranges_for(self, items, unit):
@@ -159,7 +160,7 @@ def pack(entries, start_lengths, device, staging=None):
         slots=dev[o:o + B], seq_starts=dev[o + B:o + 2 * B + 1],
         context_lens=dev[o + 2 * B + 1:o + 3 * B + 1], want_rows=dev[o + 3 * B + 1:o + 3 * B + 1 + R],
         num_tokens=T, num_seqs=B, max_new=max(counts), max_context=int(ctx.max()),
-        max_position=int(pos.max()), host_starts=starts.copy(), host_context=ctx.copy(), derived={},
+        max_position=int(pos.max()), host_starts=starts.copy(), host_context=ctx.copy(), host_slots=slots.copy(), derived={},
         context_bucket=bucket(int(ctx.max())), unequal=unequal_level(ctx))
 
 
@@ -209,7 +210,8 @@ class StaticDecodeMeta:
             seq_starts=d[4 * B:5 * B + 1], context_lens=d[5 * B + 1:6 * B + 1],
             want_rows=d[6 * B + 1:7 * B + 1], num_tokens=B, num_seqs=B, max_new=1, max_context=0,
             max_position=0, host_starts=np.arange(B + 1, dtype=np.int32),
-            host_context=np.zeros(B, dtype=np.int32), derived={}, context_bucket=0, static=self)
+            host_context=np.zeros(B, dtype=np.int32), host_slots=np.zeros(B, dtype=np.int32), derived={}, context_bucket=0,
+            static=self)
 
     def _range_place(self, i):
         first = 7 * self.batch_size + 1 + i * (self.batch_size + 2)
@@ -257,6 +259,7 @@ class StaticDecodeMeta:
             self.copied.record()
         m = self.meta
         m.host_context = context.copy()
+        m.host_slots = h[3 * B:4 * B].copy()
         m.max_context = int(max(start_lengths)) + 1
         m.max_position = m.max_context - 1
         m.context_bucket = bucket(m.max_context)

@@ -15,13 +15,14 @@ from .ops import _check, _stream
 
 _P, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 lib.register_signatures("attention_shared", {
-    "hb_attn_shared": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P],
+    "hb_attn_shared": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P],
 })
 
 ITEM_INTS = 8
 COLUMNS = {torch.bfloat16: 128, torch.float32: 16}      # (row, head) pairs of a kv head that an item holds at most
 F32_MOST_DIM = 256
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
+FOUR_MOST_PAGES = 8
 
 
 def supported(kv, nq, nkv, hd, dtype):
@@ -33,75 +34,94 @@ def supported(kv, nq, nkv, hd, dtype):
     return dtype == torch.float32 and hd % 4 == 0 and 0 < hd <= F32_MOST_DIM
 
 
-def plan(starts, context, sharing, group, nkv, columns, workgroups):
+def plan(starts, context, slots, sharing, group, nkv, columns, workgroups):
     """How a step is cut up. starts: the first packed row of each sequence and the last one's end; context: the positions it
-    holds after the step; sharing: a SharedPages. Returns int32 arrays (items [n, 8], order [rows], part_start
+    holds after the step; slots: theirs; sharing: a SharedPages. Returns int32 arrays (items [n, 8], order [rows], part_start
     [rows + 1], parts) and the most rows of an item; see csrc/attention_shared.hip.
 
-    A node of the sharing is cut into tiles of as many rows as fit `columns`; a tile's pages are cut into ranges that take
-    equally many steps (a step is a page for each of the waves that a workgroup's columns leave free), as many that the
-    workgroups (items x kv heads) come to about `workgroups`."""
+    A node of the sharing is cut into tiles of as many rows as fit `columns`; a tile's pages are cut into ranges of about as many pages
+    each that the workgroups (items x kv heads) come to `workgroups`, whole rounds of the waves that take them in turn. The pages
+    that a tile of more than 64 columns sees in part are items of their own."""
     starts, context = np.asarray(starts, dtype=np.int64), np.asarray(context, dtype=np.int64)
     counts = np.diff(starts)
     row_of = np.concatenate([[0], np.cumsum(counts[sharing.order])])            # a sequence's first row in the order
     order = np.concatenate([np.arange(starts[i], starts[i + 1]) for i in sharing.order])
     tall = max(1, columns // group)
-    tiles = []                                                                  # row0, rows, sequence, first page, end
+    tiles = []                                                                  # row0, rows, sequence, first page, end, first page seen in part
     for first, count, page, end in sharing.nodes:
         a, b, seq = int(row_of[first]), int(row_of[first + count]), int(sharing.order[first])
         for r in range(a, b, tall):
             n = min(tall, b - r)
-            # (a tile of a sequence's own rows ends at the last page that its last row sees)
-            last = end if end >= 0 else (int(context[seq]) - (b - (r + n)) - 1) // 64 + 1
-            if last > page:
-                tiles.append((r, n, seq, page, last))
-    tiles = np.array(tiles, dtype=np.int64)
-    row0, rows, seq, page, end = tiles.T
-    cols = rows * group
-    at_once = np.where(cols <= 32, 4, np.where(cols <= 64, 2, 1)) if columns == 128 else np.ones_like(cols)
-    pages = end - page
-    steps = max(1, -(-int((-(-pages // at_once)).sum()) * nkv // workgroups))
-    ranges = -(-pages // (at_once * steps))
-    per = -(-pages // ranges)
+            if end >= 0:
+                tiles.append((r, n, seq, page, end, end))
+                continue
+            # a tile of a sequence's own rows ends at the page of its last row; all of it is seen by all before the first row's page
+            whole, last = (int(context[seq]) - (b - r)) // 64, (int(context[seq]) - (b - (r + n)) - 1) // 64 + 1
+            if n * group > 64 and whole > page:
+                tiles.append((r, n, seq, page, whole, whole))
+                page_from = whole
+            else:
+                page_from = page
+            tiles.append((r, n, seq, page_from, last, whole))
+    row0, rows, seq, page, end, whole = np.array(tiles, dtype=np.int64).T
+    cols, pages = rows * group, end - page
+    turns = np.where(cols <= 32, 4, np.where(cols <= 64, 2, 1)) if columns == 128 else np.ones_like(cols)
+    share = max(1, -(-int(pages.sum()) * nkv // workgroups))
+    per = -(-share // turns) * turns
+    ranges = -(-pages // per)
+    per = -(-(-(-pages // ranges)) // turns) * turns
     of = np.repeat(np.arange(len(tiles)), ranges)
     nth = np.arange(len(of)) - np.repeat(np.cumsum(ranges) - ranges, ranges)
     items = np.zeros((len(of), ITEM_INTS), dtype=np.int64)
-    items[:, 0], items[:, 1], items[:, 2] = row0[of], rows[of], seq[of]
+    items[:, 0], items[:, 1], items[:, 2] = row0[of], rows[of], np.asarray(slots, dtype=np.int64)[seq[of]]
     items[:, 3] = page[of] + nth * per[of]
     items[:, 4] = np.minimum(items[:, 3] + per[of], end[of])
-    # (ranges rounded up may leave the last ones nothing)
-    items = items[items[:, 4] > items[:, 3]]
+    items[:, 6] = items[:, 4] > whole[of]
+    items = items[items[:, 4] > items[:, 3]]              # (ranges rounded up may leave the last ones nothing)
     n = items[:, 1]
     items[:, 5] = np.cumsum(n) - n
-    # the partial results of each row, in the order of its pages
+    # a row's partial results lie side by side, in the order of its pages
     total = int(n.sum())
     row = np.repeat(items[:, 0] - items[:, 5], n) + np.arange(total)
-    parts = np.argsort(row, kind="stable")
+    parts = np.empty(total, dtype=np.int64)
+    parts[np.argsort(row, kind="stable")] = np.arange(total)
     part_start = np.concatenate([[0], np.cumsum(np.bincount(row, minlength=len(order)))])
-    # the longest items first
-    waves = np.where(n * group <= 32, 4, np.where(n * group <= 64, 2, 1)) if columns == 128 else np.ones_like(n)
-    items = items[np.argsort(-(-(-(items[:, 4] - items[:, 3]) // waves)), kind="stable")]
+    # the longest items first, those over the same pages side by side
+    items = items[np.lexsort((items[:, 0], items[:, 3], items[:, 3] - items[:, 4]))]
+    most = int(n.max())
+    if columns == 128 and len(items) * nkv > workgroups:
+        # more workgroups than the GPU holds at a time: short items are a wave each
+        short = (items[:, 1] * group <= 32) & (items[:, 4] - items[:, 3] <= FOUR_MOST_PAGES)
+        alone, single = items[~short], items[short]
+        heads = np.zeros((-(-len(single) // 4), ITEM_INTS), dtype=np.int64)
+        n_items = len(alone) + len(heads)
+        heads[:, 0] = n_items + 4 * np.arange(len(heads))
+        heads[:, 1] = heads[:, 7] = 1
+        rest = np.zeros((4 * len(heads) - len(single), ITEM_INTS), dtype=np.int64)
+        items = np.concatenate([alone, heads, single, rest])
+    else:
+        n_items = len(items)
     as32 = lambda x: np.ascontiguousarray(x, dtype=np.int32)
-    return as32(items), as32(order), as32(part_start), as32(parts), int(n.max())
+    return as32(items), as32(order), as32(part_start), as32(parts), n_items, most
 
 
 class _Plan:
     """A plan on the GPU."""
 
-    def __init__(self, arrays, max_rows, device):
+    def __init__(self, arrays, n_items, max_rows, device):
         items, order, part_start, parts = arrays
         both = send(np.concatenate([a.ravel() for a in arrays]), device)
         at = np.cumsum([a.size for a in arrays])
         self.items, self.order, self.part_start, self.parts = both[:at[0]], both[at[0]:at[1]], both[at[1]:at[2]], both[at[2]:]
-        self.n_items, self.n_parts, self.max_rows = len(items), len(parts), max_rows
+        self.n_items, self.n_parts, self.max_rows = n_items, len(parts), max_rows
 
 
 def _plan_of(meta, nq, nkv, dtype):
     key = ("shared_plan", nq // nkv, nkv, dtype)
     found = meta.derived.get(key)          # every layer's attention asks: worked out once a step
     if found is None:
-        *arrays, max_rows = plan(meta.host_starts, meta.host_context, meta.shared, nq // nkv, nkv, COLUMNS[dtype], WORKGROUPS[dtype])
-        found = meta.derived[key] = _Plan(arrays, max_rows, meta.positions.device)
+        *arrays, n_items, max_rows = plan(meta.host_starts, meta.host_context, meta.host_slots, meta.shared, nq // nkv, nkv, COLUMNS[dtype], WORKGROUPS[dtype])
+        found = meta.derived[key] = _Plan(arrays, n_items, max_rows, meta.positions.device)
     return found
 
 
@@ -121,7 +141,6 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     _check(kv.k, "key pages", None, (pages, nkv, 64, hd))
     _check(kv.v, "value pages", kv.k.dtype, (pages, nkv, hd, 64))
     _check(kv.page_table, "page_table", torch.int32, (None, None))
-    _check(meta.slots, "slots", torch.int32, (meta.num_seqs,))
     _check(meta.positions, "positions", torch.int32, (T,))
     if sinks is not None:
         _check(sinks, "sinks", torch.float32, (nq,))
@@ -129,6 +148,6 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
     lib.call("attention_shared", "hb_attn_shared", q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), out.data_ptr(), ops.dtype_code(q),
              po.data_ptr(), pml.data_ptr(), p.items.data_ptr(), p.n_items, p.max_rows, p.order.data_ptr(), p.part_start.data_ptr(),
-             p.parts.data_ptr(), T, meta.positions.data_ptr(), meta.slots.data_ptr(), kv.page_table.data_ptr(),
+             p.parts.data_ptr(), T, meta.positions.data_ptr(), kv.page_table.data_ptr(),
              kv.page_table.shape[1], nq, nkv, hd, float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
              _stream())

@@ -99,22 +99,31 @@ def test_items_cover_what_every_row_sees_once(seed):
     starts = np.concatenate([[0], np.cumsum(news)])
     context = [h + n for h, n in zip(held, news)]
     for columns, group, nkv in ((128, 4, 8), (128, 1, 2), (128, 32, 1), (128, 7, 4), (16, 2, 4), (16, 16, 1), (16, 24, 2)):
-        items, order, part_start, parts, most = shared.plan(starts, context, found, group, nkv, columns, 512)
+        items, order, part_start, parts, n_items, most = shared.plan(starts, context, np.arange(len(held))[::-1], found, group, nkv, columns, 512)
+        fours = items[:n_items][items[:n_items, 7] == 1]                # (each stands for four that lie behind)
+        assert sorted(i for f in fours[:, 0] for i in range(f, f + 4)) == list(range(n_items, len(items)))
+        assert not items[n_items:, 7].any() and (items[n_items:, 1] * group <= 32).all()
+        items = np.concatenate([items[:n_items][items[:n_items, 7] == 0], items[n_items:]])
+        items = items[items[:, 1] > 0]
         assert sorted(order.tolist()) == list(range(starts[-1]))
         assert most == items[:, 1].max() and (most * group <= columns or (most == 1 and columns == 16))
-        pieces, owner = {}, {}
-        for row0, rows, seq, page, end, part0 in items[:, :6].tolist():
+        pieces, owner, listed = {}, {}, set()
+        for row0, rows, slot, page, end, list0, masked in items[:, :7].tolist():
             assert rows > 0 and end > page >= 0 and 0 <= row0 and row0 + rows <= len(order)
+            firsts = [held[i] + int(order[row0 + r]) - starts[i] for r in range(rows)
+                      for i in [int(np.searchsorted(starts, order[row0 + r], side="right")) - 1]]
+            assert masked or min(firsts) >= 64 * end - 1            # whoever looks at no mask sees all
             for r in range(rows):
                 token = int(order[row0 + r])
                 i = int(np.searchsorted(starts, token, side="right")) - 1
-                assert (table[i, page:end] == table[seq, page:end]).all() and end <= -(-context[i] // 64)
+                assert (table[i, page:end] == table[len(held) - 1 - slot, page:end]).all() and end <= -(-context[i] // 64)
                 pieces.setdefault(token, []).append((page, end))
-                assert part0 + r not in owner
-                owner[part0 + r] = token
+                assert list0 + r not in listed and parts[list0 + r] not in owner
+                listed.add(list0 + r)
+                owner[parts[list0 + r]] = token
         assert sorted(owner) == list(range(len(parts)))
         for t, token in enumerate(order.tolist()):
-            assert [owner[p] for p in parts[part_start[t]:part_start[t + 1]]] == [token] * (part_start[t + 1] - part_start[t])
+            assert [owner[p] for p in range(part_start[t], part_start[t + 1])] == [token] * (part_start[t + 1] - part_start[t])
             i = int(np.searchsorted(starts, token, side="right")) - 1
             position, at = held[i] + token - starts[i], 0
             for page, end in sorted(pieces[token]):
@@ -144,7 +153,7 @@ def test_what_the_shared_attention_refuses():
 
 def call(**changed):
     args = dict(q=None, k=None, v=None, out=None, dtype=1, po=None, pml=None, items=None, n_items=1, max_rows=1, order=None, start=None,
-                parts=None, n_rows=1, positions=None, slots=None, table=None, max_pages=1, nq=4, nkv=2, hd=64, scale=0.1, softcap=0.0,
+                parts=None, n_rows=1, positions=None, table=None, max_pages=1, nq=4, nkv=2, hd=64, scale=0.1, softcap=0.0,
                 sinks=None, stream=None)
     args.update(changed)
     lib.call("attention_shared", "hb_attn_shared", *args.values())
@@ -154,7 +163,7 @@ def call(**changed):
     ({"nq": 5}, "do not group"), ({"n_rows": 0}, "empty"), ({"n_items": 0}, "empty"), ({"hd": 96}, "32, 64 or 128"), ({"dtype": 7}, "dtype"),
     ({"max_rows": 65}, "exceed 128 columns"), ({"scale": 0.0}, "positive"), ({"softcap": -1.0}, "positive"),
     ({"scale": float("nan")}, "positive"), ({"n_rows": 1 << 30}, "exceed|too many rows"), ({"n_items": 1 << 30}, "too many items"),
-    ({"dtype": 0, "hd": 62}, "whole quads"), ({"dtype": 0, "hd": 260}, "up to 256"), ({"dtype": 0, "k": 8}, "16-byte"),
+    ({"dtype": 0, "hd": 62}, "whole quads"), ({"dtype": 0, "hd": 260}, "up to 256"), ({"dtype": 0, "k": 8}, "16-byte"), ({"q": 2}, "16-byte"), ({"v": 24}, "16-byte"),
     ({"dtype": 0, "n_items": 1 << 30}, "too many items")])
 def test_calls_that_the_entry_refuses(changed, text):
     with pytest.raises(BackendError, match=text):
