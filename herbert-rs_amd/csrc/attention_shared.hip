@@ -117,23 +117,22 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) qreg[t][s] = *(const bf16x8*)(qrow + s * 32);
     }
-    int seen_last = 0x7ffffffe;
-    bool alike = true;                                    // all columns see the same keys
+    int seen_last = 0x7ffffffe, seen_by_all = 0x7ffffffe;
     if (it.masked) {
-        int seen_first = 0x7ffffffe;
         seen_last = -1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             pos[t] = A.positions[token[t]];
             seen_last = max(seen_last, pos[t]);
-            seen_first = min(seen_first, pos[t]);
+            seen_by_all = min(seen_by_all, pos[t]);
         }
 #pragma unroll
         for (int off = 1; off < 16; off <<= 1) {
             seen_last = max(seen_last, __shfl_xor(seen_last, off, 64));
-            seen_first = min(seen_first, __shfl_xor(seen_first, off, 64));
+            seen_by_all = min(seen_by_all, __shfl_xor(seen_by_all, off, 64));
         }
-        alike = seen_first == seen_last;
+        // (columns of one position: what the last of them does not see, no column sees, and the sums of all are spoiled alike)
+        if (seen_by_all == seen_last) seen_by_all = 0x7ffffffe;
     }
     f32x4 oacc[NT][BLOCKS];
     float m[NT], l[NT];
@@ -198,14 +197,7 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
         u32x4 keep;
 #pragma unroll
         for (int i = 0; i < 4; ++i) keep[i] = seen >= 2 * i + 2 ? 0xffffffffu : seen == 2 * i + 1 ? 0xffffu : 0u;
-        uint32_t odd = 0;              // (an exponent of ones: its lowest bit added carries into the sign's place; two numbers a word)
-        if (!alike)
-#pragma unroll
-            for (int d = 0; d < BLOCKS; ++d)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    odd |= (((__builtin_bit_cast(u32x4, v[d])[i] & keep[i]) & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
-        if (__builtin_amdgcn_ballot_w64(odd != 0) == 0) {
+        if (key0 + 31 <= seen_by_all) {
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d) {
                 const bf16x8 clean = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, v[d]) & keep);
@@ -215,7 +207,8 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
         } else {
             // What is left that is not finite is taken out of the product, and the columns that see it get what their sums would
             // be: a second product counts, for every entry and column, the keys whose value is +inf (1 each), -inf (128) or NaN
-            // (16384; of 32 keys no count runs into the next).
+            // (16384; of 32 keys no count runs into the next). (An exponent of ones: its lowest bit added carries into the
+            // sign's place; two numbers a word.)
             bf16x8 sees[NT];
 #pragma unroll
             for (int t = 0; t < NT; ++t)
