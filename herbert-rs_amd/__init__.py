@@ -7,8 +7,8 @@ from . import config, weights, cache, parts, models
 from .config import BozasunConfig, FigalornConfig, MefatarConfig, ModasunConfig, MutedraConfig, Qwen3Config, VipalornConfig, load_config, register_architecture
 from .engine import Engine, StepEntry
 from .sampling import SamplingParams
-from .api import generate, load, write_random_model
+from .api import generate, load, score, write_random_model
 
 __all__ = ["BackendError", "BozasunConfig", "CacheError", "ConfigError", "Engine", "HerbertError", "ModelLoadError",
            "FigalornConfig", "MefatarConfig", "ModasunConfig", "MutedraConfig", "Qwen3Config", "RequestError", "SamplingParams", "StepEntry", "VipalornConfig", "generate", "load",
-           "load_config", "register_architecture", "write_random_model"]
+           "load_config", "register_architecture", "score", "write_random_model"]

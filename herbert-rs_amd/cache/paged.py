@@ -15,6 +15,10 @@ everywhere. Rows that fill a step up to a fixed size (a decode step that is
 replayed as a graph of the next larger batch size) write and read there and
 nowhere else; no sequence ever holds either.
 
+Slots may share pages: `Cache.fork` makes slots that hold what another one holds, and a page of keys and values then has several
+holders. It is never written while it has: the page that a slot's next position falls into is copied first, if others
+hold it too (`KVGroup.own`), and a page goes back to the pool with its last holder. Fixed-size state is copied when the fork is made.
+
 Per slot the host keeps the length (positions held = next position), as the
 reference keeps `seq_len` beside its storage
 (crates/backends/backend_common/src/kv_cache.rs:270-273).
@@ -27,7 +31,11 @@ import torch
 from ..errors import CacheError
 from ..hosted import send
 from .needs import KVNeed, StateNeed
+from .sharing import shared_pages
 from .slots import PAGE_TOKENS, FreeList, pages_for
+
+
+COPIED_AT_ONCE = 8       # pages (of every layer of a group) that are copied together when a slot gets its own
 
 
 @dataclass
@@ -63,6 +71,7 @@ class KVGroup:
         self.kept = pages_for(need.keep_first) if need.window else 0
         self.first_page = np.zeros(n_slots, dtype=np.int64)
         self.held_end = [0] * n_slots
+        self.further = {}        # page -> how many slots hold it beside the first, for pages that several hold
 
     def view(self, entry):
         i = self.entries.index(entry)
@@ -72,6 +81,71 @@ class KVGroup:
         if self.need.values:
             v = self.pool[i, 1].view(n_pages, self.need.kv_heads, self.need.head_dim, PAGE_TOKENS)
         return LayerKV(k, v, self.table, PAGE_TOKENS, int(self.need.window or 0))
+
+    def _give_back(self, page):
+        """One holder less; the last one's page goes back to the pool."""
+        others = self.further.get(page, 0)
+        if others > 1:
+            self.further[page] = others - 1
+        elif others == 1:
+            del self.further[page]
+        else:
+            self.pages.give_back(page)
+
+    def _written(self, slot, length):
+        """The page that the position `length` of a slot falls into, if the slot holds it already (else -1)."""
+        if length % PAGE_TOKENS == 0 or length // PAGE_TOKENS >= self.held_end[slot]:
+            return -1
+        return int(self.table_host[slot][length // PAGE_TOKENS])
+
+    def copies_missing(self, written):
+        """How many pages `own(written)` would take."""
+        if not self.further:
+            return 0
+        holders = {}
+        for slot, length in written:
+            page = self._written(slot, length)
+            if page in self.further:
+                holders[page] = holders.get(page, 0) + 1
+        return sum(min(n, self.further[page]) for page, n in holders.items())
+
+    def own(self, written):
+        """A page of its own, with the same contents, for every (slot, length) whose next position falls into one that others hold too."""
+        if not self.further:
+            return
+        pairs, left = [], {}                        # (slot, the page's place, page, its copy)
+        try:
+            for slot, length in written:
+                page = self._written(slot, length)
+                if left.get(page, self.further.get(page, 0)) > 0:
+                    pairs.append((slot, length // PAGE_TOKENS, page, self.pages.take()))
+                    left[page] = left.get(page, self.further.get(page, 0)) - 1
+            # a few pages at a time: they pass through memory of their own
+            for i in range(0, len(pairs), COPIED_AT_ONCE):
+                source, target = send(np.array([(p[2], p[3]) for p in pairs[i:i + COPIED_AT_ONCE]], dtype=np.int64).T, self.table.device)
+                self.pool.index_copy_(2, target, self.pool.index_select(2, source))
+            if pairs:
+                places, pages = send(np.array([(slot * self.pages_per_slot + at, copy) for slot, at, _, copy in pairs], dtype=np.int64).T,
+                                     self.table.device)
+                self.table.view(-1).index_copy_(0, places, pages.to(torch.int32))
+        except Exception:
+            for _, _, _, copy in pairs:
+                self.pages.give_back(copy)
+            raise
+        for slot, at, page, copy in pairs:
+            self.table_host[slot][at] = copy
+            self._give_back(page)
+
+    def fork(self, slot, new_slots):
+        """The new slots hold the pages that `slot` holds."""
+        row = self.table_host[slot]
+        rows, device_row = send(np.array(new_slots, dtype=np.int64), self.table.device), send(np.maximum(row, 0)[None], self.table.device)
+        self.table.index_copy_(0, rows, device_row.expand(len(new_slots), -1).contiguous())
+        for new in new_slots:
+            self.table_host[new] = row
+            self.first_page[new], self.held_end[new] = self.first_page[slot], self.held_end[slot]
+        for page in row[row >= 0].tolist():
+            self.further[page] = self.further.get(page, 0) + len(new_slots)
 
     def pages_missing(self, slot, new_length):
         """How many pages `ensure(slot, new_length)` would take."""
@@ -106,7 +180,7 @@ class KVGroup:
         p = int(self.first_page[slot])
         while (p + 1) * PAGE_TOKENS <= oldest:
             if row[p] >= 0 and p >= self.kept:
-                self.pages.give_back(int(row[p]))
+                self._give_back(int(row[p]))
                 row[p] = -1
             p += 1
         self.first_page[slot] = p
@@ -127,14 +201,14 @@ class KVGroup:
             raise CacheError("cannot roll a windowed cache back past keys it has given up")
         for p in range(pages_for(length), self.held_end[slot]):
             if row[p] >= 0:
-                self.pages.give_back(int(row[p]))
+                self._give_back(int(row[p]))
                 row[p] = -1
         self.held_end[slot] = min(self.held_end[slot], pages_for(length))
 
     def free_slot(self, slot):
         row = self.table_host[slot]
         for p in np.nonzero(row >= 0)[0]:
-            self.pages.give_back(int(row[p]))
+            self._give_back(int(row[p]))
         row[:] = -1
         self.first_page[slot] = 0
         self.held_end[slot] = 0
@@ -169,6 +243,7 @@ class Cache:
         self.slots = FreeList(self.n_slots, "slot")
         self.lengths = np.zeros(self.n_slots, dtype=np.int64)
         self._taken = set()      # slots taken whose state is still to be cleared
+        self.sharing_version = 0     # another whenever slots may have come to share other pages
         self._saved_slots = (None, None)    # the slots that save_state was last asked for and the stream, and their numbers on the GPU
         self.kv_groups = {}
         self.state_groups = {}
@@ -227,6 +302,48 @@ class Cache:
             self._taken.add(slot)
         return slot
 
+    def fork(self, slot, count=1):
+        """`count` new slots that hold what `slot` holds: its positions, in the same pages, and a copy of its fixed-size state. All or none:
+        where slots are missing CacheError is raised and nothing has changed."""
+        length, count = self.length(slot), int(count)
+        if count < 1:
+            raise CacheError(f"a slot is forked into one or more, not {count}")
+        if count > self.slots.free_count:
+            raise CacheError(f"a fork into {count} slots but only {self.slots.free_count} of {self.n_slots} are free")
+        self.clear_taken()
+        new_slots, held = [self.slots.take() for _ in range(count)], []
+        try:
+            for g in self.state_groups.values():
+                at = send(np.array(new_slots, dtype=np.int64), g.data.device)
+                one = g.data[:, slot:slot + 1]
+                g.data.index_copy_(1, at, one.expand(one.shape[0], count, *one.shape[2:]).clone(memory_format=torch.contiguous_format))
+            for g in self.kv_groups.values():
+                g.fork(slot, new_slots)
+                held.append(g)
+        except Exception:
+            for new in new_slots:
+                self.slots.give_back(new)
+                for g in held:
+                    g.free_slot(new)
+            raise
+        for new in new_slots:
+            self.lengths[new] = length
+        self.sharing_version += 1
+        return new_slots
+
+    @property
+    def shares_pages(self):
+        """True while some page has several holders."""
+        return any(g.further for g in self.kv_groups.values())
+
+    def shared_pages(self, slots, held):
+        """The SharedPages of a step's sequences by their slots and the positions they hold before it; None where they share
+        none. Of a group without a window: slots share the same places of every such group."""
+        for g in self.kv_groups.values():
+            if not g.need.window and g.further:
+                return shared_pages(g.table_host[np.asarray(slots, dtype=np.int64)], held)
+        return None
+
     def clear_taken(self):
         """Clear the state of the slots that were taken since the last call. Whoever is to read or write state calls it, and
         so does whoever makes room for a step: views of the state may be held from before."""
@@ -258,6 +375,7 @@ class Cache:
 
     def free_slot(self, slot):
         self.slots.give_back(slot)
+        self.sharing_version += 1
         for g in self.kv_groups.values():
             g.free_slot(slot)
         self.lengths[slot] = 0
@@ -276,6 +394,9 @@ class Cache:
             raise CacheError(f"slot {slot}: {new_length} positions exceed the model's "
                              f"{self.max_positions}")
         for g in self.kv_groups.values():
+            if new_tokens and g.further:
+                g.own([(slot, self.length(slot))])
+                self.sharing_version += 1
             g.ensure([(slot, new_length)])
         return new_length
 
@@ -284,18 +405,24 @@ class Cache:
         group needs are counted first, and a step that does not fit raises CacheError with the
         cache unchanged."""
         self.clear_taken()
-        targets = []
+        targets, written = [], []
         for slot, new_tokens in wanted:
             new_length = self.length(slot) + int(new_tokens)
             if new_length > self.max_positions:
                 raise CacheError(f"slot {slot}: {new_length} positions exceed the model's "
                                  f"{self.max_positions}")
             targets.append((slot, new_length))
+            if new_tokens:
+                written.append((slot, new_length - int(new_tokens)))
         for g in self.kv_groups.values():
-            need = sum(g.pages_missing(slot, n) for slot, n in targets)
+            need = sum(g.pages_missing(slot, n) for slot, n in targets) + g.copies_missing(written)
             if need > g.pages.free_count:
                 raise CacheError(f"the step needs {need} more pages of {PAGE_TOKENS} tokens but only "
                                  f"{g.pages.free_count} of {g.pages.count} are free")
+        if self.shares_pages:
+            self.sharing_version += 1 if any(g.copies_missing(written) for g in self.kv_groups.values()) else 0
+            for g in self.kv_groups.values():
+                g.own(written)
         for g in self.kv_groups.values():
             g.ensure(targets)
 
@@ -352,6 +479,7 @@ class Cache:
         for g in self.kv_groups.values():
             g.truncate(slot, length)
         self.lengths[slot] = length
+        self.sharing_version += 1
 
     # ---- views for the parts
     def kv_view(self, entry):
@@ -366,10 +494,10 @@ class Cache:
         self.slots.check()
         for g in self.kv_groups.values():
             g.pages.check()
-            held = g.table_host[g.table_host >= 0]
-            if len(set(held.tolist())) != len(held):
-                raise CacheError("a page is in two places of the page table")
-            if len(held) != g.pages.held_count:
+            held, holders = np.unique(g.table_host[g.table_host >= 0], return_counts=True)
+            if any(n != 1 + g.further.get(page, 0) for page, n in zip(held.tolist(), holders.tolist())):
+                raise CacheError("a page is in more or fewer places of the page table than slots hold it")
+            if len(held) != g.pages.held_count or not set(g.further) <= set(held.tolist()):
                 raise CacheError("held pages and the page table disagree")
             for slot in range(self.n_slots):
                 if not self.slots.is_held(slot) and (g.table_host[slot] >= 0).any():

@@ -3,7 +3,7 @@
 Slots that were forked from one another name the same pages at the beginning of their page tables. The reference keeps
 a cache a sequence (crates/backends/backend_common/src/kv_cache.rs:270-273) and shares nothing.
 """
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import List, Tuple
 
 import numpy as np
@@ -20,6 +20,17 @@ class SharedPages:
     of the sequence's pages. Every page of a sequence lies in exactly one of the nodes that it is in."""
     order: np.ndarray
     nodes: List[Tuple[int, int, int, int]]
+    _filled: object = field(default=None, repr=False, compare=False)
+
+    def filled_up(self, sequences):
+        """The same of a step that is filled up to so many sequences: each of the further ones by itself."""
+        n = len(self.order)
+        if sequences == n:
+            return self
+        if self._filled is None or len(self._filled.order) != sequences:
+            more = range(n, sequences)
+            self._filled = SharedPages(np.concatenate([self.order, np.array(more, dtype=np.int64)]), self.nodes + [(i, 1, 0, -1) for i in more])
+        return self._filled
 
     @property
     def pages_saved(self):

@@ -4,7 +4,7 @@ Kept with their names, meanings and defaults: --model, --prompt, --prompt-file, 
 --max-tokens (2048), --ignore-eos, --no-repeat-check, --stop, --verbose, --temperature (0.4,
 0 = greedy), --top-k (40, 0 = off), --top-p (0.9, 1.0 = off), --show-specials, --backend (one
 backend here; `help` lists it) and --gpu (an index, or `list`). Added here:
---dtype, --seed, --cache-tokens, and --random-weights to write a random model folder.
+--dtype, --seed, --cache-tokens, --samples, --logprobs, and --random-weights to write a random model folder.
 With a tokenizer.json in the model folder the prompt is text wrapped in the architecture's
 chat template (for this family ChatML, main.rs:281-294; the template and the end-of-turn
 token are data of the architecture's registry entry); without one it is comma-separated
@@ -18,6 +18,7 @@ once with 130 (main.rs:22-50,1242-1245). Without --prompt and --prompt-file the 
 of `chat.py` starts (main.rs:70,718-757), which needs a tokenizer.
 """
 import argparse
+import io
 import os
 import signal
 import sys
@@ -224,6 +225,9 @@ def make_parser():
     ap.add_argument("--prefill-chunk-size", type=int, default=None,
                     help="Process the prompt in chunks of N tokens (default: HERBERT_PREFILL_CHUNK_SIZE, else whole)")
     ap.add_argument("--seed", type=int, default=None, help="Sampler seed (default: from the clock)")
+    ap.add_argument("--samples", type=int, default=1, help="So many answers to the prompt, which goes through the model once")
+    ap.add_argument("--logprobs", type=int, default=None, metavar="N",
+                    help="After the answer, a line a token: id, log probability, entropy and N alternatives")
     ap.add_argument("--dtype", choices=["bfloat16", "float32"], default="bfloat16")
     ap.add_argument("--cache-tokens", type=int, default=None,
                     help="tokens the cache holds (default: prompt + max-tokens)")
@@ -295,6 +299,8 @@ def _run(args):
         if tokenizer is None or chat is None:
             raise RequestError("--prompt or --prompt-file is required: the conversation needs a tokenizer.json "
                                "and a chat template")
+        if args.samples != 1 or args.logprobs is not None:
+            raise RequestError("--samples and --logprobs go with a prompt, not with a conversation")
         from .chat import run_from_args
         return run_from_args(args, tokenizer, chat, system, prefill_chunk)
     if tokenizer is not None:
@@ -318,31 +324,46 @@ def _run(args):
     think_tokens = think_tokens_of(chat, tokenizer) if think_budget > 0 else None
 
     t0 = time.perf_counter()
-    cache_tokens = args.cache_tokens or (len(ids) + args.max_tokens + 65)
+    samples = args.samples
+    if samples < 1:
+        raise RequestError("--samples must be at least 1")
+    cache_tokens = args.cache_tokens or (len(ids) + args.max_tokens + 65 + (samples - 1) * (args.max_tokens + 192))
     engine = load(args.model, dtype=args.dtype, cache_tokens=cache_tokens)
     load_seconds = time.perf_counter() - t0
 
     params = SamplingParams(temperature=args.temperature, top_k=args.top_k, top_p=args.top_p,
                             max_tokens=args.max_tokens + 1, stop_ids=tuple(stop_ids),
                             ignore_eos=args.ignore_eos, repeat_check=not args.no_repeat_check,
-                            seed=args.seed, think_budget=think_budget, think_tokens=think_tokens)
+                            seed=args.seed, think_budget=think_budget, think_tokens=think_tokens, samples=samples,
+                            logprobs=args.logprobs)
     check_think_tokens(think_tokens, engine.spec.vocab_size)
-    on_token = StreamPrinter(tokenizer, args.show_specials, stop_strings).on_token
+    # (several answers run side by side: they are printed when they are done, one after the other)
+    printers = [StreamPrinter(tokenizer, args.show_specials, stop_strings, io.StringIO() if samples > 1 else None) for _ in range(samples)]
+
+    def on_token(i, tok):
+        return printers[i].on_token(i, tok)
 
     interrupt = InterruptFlag().install()
     t0 = time.perf_counter()
     try:
-        result = engine.generate([ids], params, on_token=on_token, interrupt=interrupt,
-                                 prefill_chunk=prefill_chunk)[0]
+        results = engine.generate([ids], params, on_token=on_token, interrupt=interrupt, prefill_chunk=prefill_chunk)
     finally:
         interrupt.restore()
     total = time.perf_counter() - t0
-    print()
-    if result.stop_reason == INTERRUPTED:
+    if samples == 1:
+        print()
+    for i, result in enumerate(results):
+        if samples > 1:
+            print(f"--- {i + 1} ---\n{printers[i].out.getvalue()}")
+        for t in result.logprobs or ():
+            others = " ".join(f"{tok}:{lp:.4f}" for tok, lp in t.top)
+            print(f"{t.token}\t{t.logprob:.4f}\t{t.entropy:.4f}" + (f"\t{others}" if others else ""))
+    result = results[0]
+    if any(r.stop_reason == INTERRUPTED for r in results):
         print("[herbert] Interrupted", file=sys.stderr)
     if args.verbose:
         st = engine.last_generation_stats
-        decoded = max(0, st.generated_tokens - 1)
+        decoded = max(0, st.generated_tokens - samples)
         err = sys.stderr
         print("--- Stats ---", file=err)
         print(f"Backend:         {BACKEND}", file=err)

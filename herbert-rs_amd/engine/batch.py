@@ -199,6 +199,7 @@ class StaticDecodeMeta:
         self.host = torch.zeros(size, dtype=torch.int32, pin_memory=torch.device(device).type == "cuda")
         self.copied = None       # event after the last copy out of `host`
         self.dev = torch.zeros(size, dtype=torch.int32, device=device)
+        self.shared_plans = {}   # kind of heads -> (plan of the shared attention in fixed buffers, whether it pays)
         self.range_lists = []    # (items, unit) of the lists handed out, in the order of their places
         h = self.host_array = self.host.numpy()
         h[2 * B:3 * B] = np.arange(B)            # seq_of
@@ -212,6 +213,27 @@ class StaticDecodeMeta:
             max_position=0, host_starts=np.arange(B + 1, dtype=np.int32),
             host_context=np.zeros(B, dtype=np.int32), host_slots=np.zeros(B, dtype=np.int32), derived={}, context_bucket=0,
             static=self)
+
+    def shared_plan(self, key, make, pays):
+        """The plan of the shared attention for heads of one kind (key), in buffers that stay where they are (`make` makes them, at the
+        first call, not while a graph is recorded), or None where it does not pay (`pays(meta)`)."""
+        found = self.shared_plans.get(key)
+        if found is None:
+            if self.dev.is_cuda and torch.cuda.is_current_stream_capturing():
+                from ..errors import NeedsEagerStep
+                raise NeedsEagerStep("a plan of shared pages is first asked for while a graph is recorded")
+            found = self.shared_plans[key] = (make(self.batch_size, self.dev.device), pays)
+            if pays(self.meta):
+                found[0].refill(self.meta)
+        return found[0] if found[1](self.meta) else None
+
+    @property
+    def shared_shape(self):
+        """What a recorded step with shared pages is tied to beside its batch size and contexts; None where no pages are shared to
+        any use."""
+        if self.meta.shared is None:
+            return None
+        return tuple((key, plan.shape if pays(self.meta) else None) for key, (plan, pays) in self.shared_plans.items())
 
     def _range_place(self, i):
         first = 7 * self.batch_size + 1 + i * (self.batch_size + 2)
@@ -232,7 +254,8 @@ class StaticDecodeMeta:
         self.dev[place].copy_(self.host[place])
         return self.dev[place]
 
-    def update(self, entries, start_lengths):
+    def update(self, entries, start_lengths, shared=None):
+        """shared: the pages that the entries' sequences hold together (cache.SharedPages), if any."""
         B, n = self.batch_size, len(entries)
         if n > B:
             raise ValueError(f"{n} sequences do not fit a step of {B}")
@@ -265,4 +288,11 @@ class StaticDecodeMeta:
         m.context_bucket = bucket(m.max_context)
         m.unequal = unequal
         m.num_real = n
+        m.shared = None if shared is None else shared.filled_up(B)
+        if shared is not None:
+            if self.shared_plans and not any(pays(m) for _, pays in self.shared_plans.values()):
+                m.shared = None
+            for plan, pays in self.shared_plans.values():
+                if m.shared is not None and pays(m):
+                    plan.refill(m)
         return m

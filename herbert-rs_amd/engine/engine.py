@@ -14,7 +14,7 @@ from collections import OrderedDict
 import numpy as np
 import torch
 
-from ..cache import Cache
+from ..cache import PAGE_TOKENS, Cache, pages_for
 from ..config import load_config
 from ..errors import BackendError, ModelLoadError, NeedsEagerStep, RequestError
 from ..parts import Runtime
@@ -51,6 +51,8 @@ MAX_GRAPHS = 192
 # slots need, if fewer; a larger batch makes a larger one (twice the rows, or what the batch needs)
 # and every graph, which holds the old one's address, is dropped.
 SHARED_LOGITS_ROWS = 64
+# Rows of logits that scoring asks for in one step (311 MB for a vocabulary of 151,936).
+SCORED_ROWS = 512
 # Batch sizes whose fixed metadata buffers are kept; the least recently used goes, with its graphs.
 MAX_DECODE_BATCH_SIZES = 96
 
@@ -83,11 +85,12 @@ class Engine:
         self.static_decode = self.model.graph_safe
         self.use_graphs = bool(use_graphs) and self.model.graph_safe
         self._decode = OrderedDict()    # batch size -> _DecodeState, least recently used first
-        self._graphs = OrderedDict()    # (batch size, context bucket, unequal) -> graph, least recently used first
+        self._graphs = OrderedDict()    # (batch size, context bucket, unequal, shared plan's shape) -> graph, least recently used first
         self._shared_logits = None      # [rows, vocab], made by the first decode step, grown by a larger batch
         self._capture_stream = None     # the stream that graphs are captured on
         self._sized_rows = 0            # the largest decode step that has run outside a graph: buffers for it exist
         self.graphs_captured = 0
+        self._sharing = (None, None)    # (the cache's version of what is shared, slots) of a step, its SharedPages
         self.ignored_tensors = []       # stored tensors that the model did not ask for
         self._tensor_source = None      # how get_tensor finds a tensor again: set by the constructors below
 
@@ -156,6 +159,22 @@ class Engine:
     def free_slot(self, slot):
         self.cache.free_slot(slot)
 
+    def fork(self, slot, count=1):
+        """`count` new slots that hold what `slot` holds, without a pass through the model: they share its pages of keys and values
+        (a page is copied when one of its holders writes into it) and have copies of its fixed-size state. Where slots of one step
+        share pages, an attention that sees whole contexts reads those once for all of them. The reference has one cache a sequence
+        and runs a prompt again for every answer to it (crates/backends/backend_common/src/kv_cache.rs:270-273)."""
+        return self.cache.fork(slot, count)
+
+    def _shared_pages(self, entries, starts):
+        """The pages that the sequences of a step share (kept while the same slots go on sharing the same ones)."""
+        if len(entries) < 2 or not self.cache.shares_pages:
+            return None
+        key = (self.cache.sharing_version, tuple(e.slot for e in entries))
+        if self._sharing[0] != key:
+            self._sharing = (key, self.cache.shared_pages(key[1], starts))
+        return self._sharing[1]
+
     def truncate(self, slot, length):
         """Roll a sequence back to its first `length` positions; the next step's tokens go on from
         there and overwrite what lay behind (the reference's truncate_kv,
@@ -223,6 +242,7 @@ class Engine:
         # nothing that can fail follows it: the caller's copy has its memory before; a sequence's
         # first step found zeros; nothing for a cache without state)
         state_before = []
+        shared = self._shared_pages(entries, starts)
 
         def set_aside():
             held = [e.slot for e, start in zip(entries, starts) if start]
@@ -231,12 +251,13 @@ class Engine:
         try:
             if self.static_decode and all(len(e.tokens) == 1 and list(e.want) == [0] for e in entries):
                 own = torch.empty((len(entries), vocab), dtype=torch.float32, device=self.device) if keep_logits else None
-                logits = self._decode_step(entries, starts, tokens_on_device, set_aside)
+                logits = self._decode_step(entries, starts, tokens_on_device, set_aside, shared)
                 if keep_logits:
                     logits = own.copy_(logits)
             else:
                 set_aside()
                 meta = batching.pack(entries, starts, self.device)
+                meta.shared = shared
                 if tokens_on_device is not None:
                     meta.token_ids.copy_(tokens_on_device)
                 logits = self.model.forward(self.rt, meta, self.cache)
@@ -251,7 +272,7 @@ class Engine:
         self.steps_run += 1
         return logits
 
-    def _decode_step(self, entries, starts, tokens_on_device, set_aside):
+    def _decode_step(self, entries, starts, tokens_on_device, set_aside, shared=None):
         """One token for each sequence, every logit wanted: the launch-bound case. The step's
         metadata lives in fixed buffers, and the forward pass of a shape is recorded into a HIP graph
         that is replayed from then on, so that the host launches one graph and not hundreds of
@@ -259,8 +280,8 @@ class Engine:
         (batch.decode_batch_bucket), filled up with padding rows in the cache's padding slot: a batch
         whose sequences end one after another then meets few new shapes instead of one a sequence.
         A graph is tied to that batch size, to the bucket of the longest context (which sizes the
-        attention grid) and to whether the contexts are of very unequal lengths (the attention then
-        deals its grid out by a list). All graphs write their logits into the first rows of the
+        attention grid), to whether the contexts are of very unequal lengths (the attention then
+        deals its grid out by a list) and, where sequences share pages, to the size of that plan. All graphs write their logits into the first rows of the
         engine's one buffer; what is returned here is a view of those rows, which the next decode
         step writes again (`step` copies it for callers that keep it). At most MAX_GRAPHS graphs and
         MAX_DECODE_BATCH_SIZES batch sizes are kept, the least recently used go first. `set_aside` is called before
@@ -286,13 +307,13 @@ class Engine:
             state = self._decode[B] = _DecodeState(StaticDecodeMeta(B, self.device, self.cache.pad_slot),
                                                    self._shared_logits[:B])
         self._decode.move_to_end(B)
-        meta = state.static.update(entries, starts)
+        meta = state.static.update(entries, starts, shared)
         if tokens_on_device is not None:
             meta.token_ids[:n].copy_(tokens_on_device)      # behind the copy from the host, before the graph
         if not self.use_graphs:
             set_aside()
             return self.model.forward(self.rt, meta, self.cache, logits_out=state.logits)[:n]
-        key = (B, meta.context_bucket, meta.unequal)
+        key = (B, meta.context_bucket, meta.unequal, state.static.shared_shape)
         graph = self._graphs.get(key)
         if graph is not None:
             self._graphs.move_to_end(key)
@@ -347,6 +368,72 @@ class Engine:
         """(graphs kept, batch sizes kept, bytes of the decode steps' logits buffers)."""
         held = 0 if self._shared_logits is None else self._shared_logits.numel() * 4
         return len(self._graphs), len(self._decode), held
+
+    def score(self, prompt, continuations, top=0):
+        """What the model says of given continuations of a prompt: for each a list with a sampling.logprobs.TokenLogprob a token
+        (log p(token | prompt, the continuation's tokens before it), the entropy there and the `top` most probable tokens).
+        The prompt goes through the model once; the continuations go on from forks of its slot, as many side by side as there
+        are slots for, and their steps read the prompt's keys and values together. A text by itself: its first token as the
+        prompt, the rest as the continuation."""
+        from ..sampling import MOST_ALTERNATIVES
+        from ..sampling.logprobs import LogprobReader
+        prompt, texts = list(prompt), [list(c) for c in continuations]
+        if not prompt or not texts or not all(texts):
+            raise RequestError("scoring needs a prompt and continuations of at least one token each")
+        if not 0 <= top <= MOST_ALTERNATIVES:
+            raise RequestError(f"top must be between 0 and {MOST_ALTERNATIVES} alternatives")
+        vocab, longest = self.spec.vocab_size, max(len(c) for c in texts)
+        for c in texts:
+            if not all(isinstance(t, (int, np.integer)) and not isinstance(t, bool) and 0 <= t < vocab for t in c):
+                raise RequestError(f"token ids must be integers below {vocab}")
+        if len(prompt) + longest - 1 > self.spec.max_positions:
+            raise RequestError(f"{len(prompt) + longest - 1} positions exceed max_position_embeddings ({self.spec.max_positions})")
+        reader = LogprobReader(top, vocab, self.device)
+        results = [[] for _ in texts]
+        first = self.alloc_slot()
+        try:
+            logits = self.step([StepEntry(first, prompt, [len(prompt) - 1])])
+            for i in range(0, len(texts), SCORED_ROWS):         # (all continuations' first tokens are scored on the same logits)
+                some = texts[i:i + SCORED_ROWS]
+                said = reader.of(logits.expand(len(some), vocab).contiguous(), [c[0] for c in some])
+                for r, one in zip(results[i:], said):
+                    r.append(one)
+            left = [i for i, c in enumerate(texts) if len(c) > 1]
+            while left:
+                # as many side by side as there are slots and pages for (one at least: what does not fit is the cache's to say)
+                now, room = [], min([g.pages.free_count for g in self.cache.kv_groups.values()] or [len(texts) * longest])
+                for i in left[:max(1, min(self.cache.slots.free_count, SCORED_ROWS))]:
+                    room -= pages_for(len(prompt) + len(texts[i]) - 1) - len(prompt) // PAGE_TOKENS
+                    if now and room < 0:
+                        break
+                    now.append(i)
+                left = left[len(now):]
+                slots = dict(zip(now, self.fork(first, len(now))))
+                try:
+                    self._score_side_by_side({i: texts[i] for i in now}, slots, reader, results)
+                finally:
+                    for slot in slots.values():
+                        self.free_slot(slot)
+        finally:
+            self.free_slot(first)
+        return results
+
+    def _score_side_by_side(self, texts, slots, reader, results):
+        """Continuations whose first tokens have been scored, through slots of their own, in steps of at most SCORED_ROWS rows."""
+        fed = {i: 0 for i in texts}
+        while fed:
+            share = max(1, SCORED_ROWS // len(fed))
+            entries, tokens = [], []
+            for i in fed:
+                piece = texts[i][fed[i]:min(fed[i] + share, len(texts[i]) - 1)]
+                entries.append(StepEntry(slots[i], piece, list(range(len(piece)))))
+                tokens += texts[i][fed[i] + 1:fed[i] + 1 + len(piece)]
+            said = iter(reader.of(self.step(entries), tokens))
+            for i, e in zip(list(fed), entries):
+                results[i] += [next(said) for _ in e.tokens]
+                fed[i] += len(e.tokens)
+                if fed[i] == len(texts[i]) - 1:
+                    del fed[i]
 
     def generate(self, prompts, params=None, max_batch=64, on_token=None, interrupt=None, prefill_chunk=None):
         """Generate from lists of token ids; see engine.generate.Generator."""

@@ -18,6 +18,10 @@ the sampler left them on the GPU, and the host reads them, applies the stop
 rules and calls `on_token` while the next step already runs. The tokens and
 stop reasons are those of the step-by-step loop.
 
+Several answers to a prompt (`SamplingParams.samples`, not in the reference) are requests of their own with generator streams of their own,
+but the prompt goes through the model once: the first answer's slot is forked for the others (`Engine.fork`), whose steps
+then read the prompt's keys and values together. With `SamplingParams.logprobs` every token comes with what its logits said of it.
+
 `max_tokens` here counts every generated token, the one the prompt's step
 gives included: the reference's chat and server loops (`for _ in
 1..max_tokens` after the first token, crates/cli/src/chat.rs:231). Its
@@ -27,7 +31,9 @@ command line here asks this loop for max_tokens + 1 to give what that gives.
 """
 import time
 from dataclasses import dataclass, field
-from typing import List
+from typing import List, Optional
+
+import torch
 
 from ..cache import PAGE_TOKENS
 from ..errors import BackendError, RequestError
@@ -41,6 +47,7 @@ class GenerationResult:
     tokens: List[int]
     stop_reason: str
     prompt_tokens: int
+    logprobs: Optional[List] = None      # a sampling.logprobs.TokenLogprob a token, where they were asked for
 
 
 @dataclass
@@ -57,24 +64,28 @@ def _rounded(n):
     return (n + PAGE_TOKENS - 1) // PAGE_TOKENS * PAGE_TOKENS
 
 
-def plan_batches(prompt_lengths, max_new, max_batch, capacity_tokens, max_positions):
-    """Lists of request indices, in order, each list one batch that fits the cache."""
+def plan_batches(prompt_lengths, max_new, max_batch, capacity_tokens, max_positions, samples=1):
+    """Lists of request indices, in order, each list one batch that fits the cache. Request i is an answer to prompt i // samples (of
+    which prompt_lengths has one length each); answers to one prompt share its whole pages within a batch."""
     batches, current, used = [], [], 0
-    for i, n in enumerate(prompt_lengths):
+    for p, n in enumerate(prompt_lengths):
         if n <= 0:
-            raise RequestError(f"request {i} has an empty prompt")
+            raise RequestError(f"request {p} has an empty prompt")
         if n > max_positions:
-            raise RequestError(f"request {i}: prompt of {n} tokens exceeds "
+            raise RequestError(f"request {p}: prompt of {n} tokens exceeds "
                                f"max_position_embeddings ({max_positions})")
-        need = _rounded(min(n + max_new, max_positions))
-        if need > capacity_tokens:
-            raise RequestError(f"request {i} needs room for {need} tokens but the cache holds "
+        whole = _rounded(min(n + max_new, max_positions))
+        if whole > capacity_tokens:
+            raise RequestError(f"request {p} needs room for {whole} tokens but the cache holds "
                                f"{capacity_tokens}")
-        if current and (len(current) >= max_batch or used + need > capacity_tokens):
-            batches.append(current)
-            current, used = [], 0
-        current.append(i)
-        used += need
+        own = whole - n // PAGE_TOKENS * PAGE_TOKENS       # beside an answer in the same batch: the prompt's last page is copied
+        for i in range(p * samples, (p + 1) * samples):
+            need = own if current and current[-1] // samples == p else whole
+            if current and (len(current) >= max_batch or used + need > capacity_tokens):
+                batches.append(current)
+                current, used, need = [], 0, whole
+            current.append(i)
+            used += need
     if current:
         batches.append(current)
     return batches
@@ -118,7 +129,8 @@ class Generator:
         self._views = {"keep_logits": False} if getattr(engine, "hands_out_copies", False) else {}
 
     def generate(self, prompts, params=None, on_token=None, interrupt=None):
-        """One GenerationResult per prompt (a list of token ids), in the prompts' order.
+        """One GenerationResult per prompt (a list of token ids), in the prompts' order; with params.samples > 1 that many for every
+        prompt, one after the other: request i is then an answer to prompt i // samples.
         on_token(request index, token) is called for every generated token; if it returns a
         string, the sequence ends there with that stop reason (the token is kept). It must not
         use the engine: the step after the token's may already be on the GPU. `interrupt()`
@@ -130,47 +142,76 @@ class Generator:
         spec = eng.spec
         capacity = eng.cache.n_pages * PAGE_TOKENS
         batches = plan_batches([len(p) for p in prompts], params.max_tokens, self.max_batch,
-                               capacity, spec.max_positions)
+                               capacity, spec.max_positions, params.samples)
+        prompts = [p for p in prompts for _ in range(params.samples)]
         chooser = self.make_chooser(params, len(prompts), spec.vocab_size, eng.device)
         results = [None] * len(prompts)
         self.stats = GenerationStats()
         for members in batches:
             if interrupt is not None and interrupt():
                 for i in members:
-                    results[i] = GenerationResult([], INTERRUPTED, len(prompts[i]))
+                    results[i] = GenerationResult([], INTERRUPTED, len(prompts[i]), None if params.logprobs is None else [])
                 continue
             self._run_batch(members, prompts, params, chooser, results, on_token, interrupt)
             self.stats.batches += 1
         return results
 
-    def _prompts(self, live, prompts, slots, chooser):
-        """The prompts of a batch through the engine; the first token of each sequence, in the
-        order of `live`. Whole in one step, or, with a prefill chunk, in steps that carry the
-        next piece of every prompt that still has one: a sequence's token is chosen in the step
-        that brings its last piece."""
-        eng, chunk = self.engine, self.prefill_chunk
-        if chunk is None or all(len(prompts[i]) <= chunk for i in live):
-            entries = [StepEntry(slots[i], list(prompts[i]), [len(prompts[i]) - 1]) for i in live]
-            return chooser.choose(eng.step(entries), list(live))
-        fed = {i: 0 for i in live}
-        first = {}
-        while len(first) < len(live):
-            entries, ending = [], []
-            for i in live:
-                left = len(prompts[i]) - fed[i]
-                if left <= 0:
-                    continue
-                n = min(chunk, left)
-                entries.append(StepEntry(slots[i], list(prompts[i][fed[i]:fed[i] + n]), [n - 1] if n == left else []))
-                if n == left:
-                    ending.append(i)
-                fed[i] += n
-            logits = eng.step(entries)
-            if ending:
-                first.update(zip(ending, chooser.choose(logits, ending)))
-        return [first[i] for i in live]
+    def _choose(self, chooser, logits, order, logprobs):
+        """Tokens of the rows of a step's logits, and what the logits said of them (None: not asked for)."""
+        if logprobs is None:
+            return chooser.choose(logits, order), None
+        if getattr(chooser, "changes_logits", False):
+            said = logits.clone()           # (as the model gave them)
+            tokens = chooser.choose(logits, order)
+            return tokens, logprobs.of(said, tokens)
+        tokens = chooser.choose(logits, order)
+        return tokens, logprobs.of(logits, tokens)
 
-    def _decode_ahead(self, live, slots, generated, params, chooser, take, kept=()):
+    def _prompts(self, live, prompts, slots, chooser, leader, logprobs):
+        """The prompts of a batch through the engine; the first token of each sequence, in the
+        order of `live`, and what the logits said of them. Whole in one step, or, with a prefill chunk, in steps that carry the
+        next piece of every prompt that still has one: a sequence's token is chosen in the step
+        that brings its last piece. leader[i]: the request whose slot the prompt of request i goes through; the others' slots are
+        forked from it."""
+        eng, chunk = self.engine, self.prefill_chunk
+        leading = [i for i in live if leader[i] == i]
+        following = {i: [j for j in live if leader[j] == i] for i in leading}         # (with itself, first)
+
+        def ended(leaders, logits):
+            order = [j for i in leaders for j in following[i]]
+            if len(order) > len(leaders):
+                rows = [r for r, i in enumerate(leaders) for _ in following[i]]
+                logits = logits[torch.tensor(rows, dtype=torch.long, device=logits.device)]
+                for i in leaders:
+                    others = following[i][1:]
+                    if others:
+                        slots.update(zip(others, eng.fork(slots[i], len(others))))
+            tokens, said = self._choose(chooser, logits, order, logprobs)
+            first.update(zip(order, zip(tokens, said if said is not None else [None] * len(order))))
+
+        first = {}
+        if chunk is None or all(len(prompts[i]) <= chunk for i in leading):
+            entries = [StepEntry(slots[i], list(prompts[i]), [len(prompts[i]) - 1]) for i in leading]
+            ended(leading, eng.step(entries))
+        else:
+            fed = {i: 0 for i in leading}
+            while len(first) < len(live):
+                entries, ending = [], []
+                for i in leading:
+                    left = len(prompts[i]) - fed[i]
+                    if left <= 0:
+                        continue
+                    n = min(chunk, left)
+                    entries.append(StepEntry(slots[i], list(prompts[i][fed[i]:fed[i] + n]), [n - 1] if n == left else []))
+                    if n == left:
+                        ending.append(i)
+                    fed[i] += n
+                logits = eng.step(entries)
+                if ending:
+                    ended(ending, logits)
+        return [first[i][0] for i in live], None if logprobs is None else [first[i][1] for i in live]
+
+    def _decode_ahead(self, live, slots, generated, params, chooser, take, kept=(), logprobs=None):
         """Decoding with the host one step behind the GPU. The tokens that a step chooses stay on
         the GPU, and the next step is put on the stream with them at once, before the host has
         seen them; the host reads a step's tokens while the next one runs, so the GPU does not
@@ -192,12 +233,14 @@ class Generator:
                        for i in order]
             logits = eng.step(entries, tokens_on_device=device_tokens, **self._views)
             self.stats.decode_steps += 1
-            return chooser.choose_ahead(logits, order), {i: eng.cache.length(slots[i]) for i in order}
+            pending = chooser.choose_ahead(logits, order)
+            said = logprobs.launch(logits, pending.device) if logprobs is not None else None
+            return pending, said, {i: eng.cache.length(slots[i]) for i in order}
 
         if not live:
             return
         order = list(live)
-        pending, held = launch(order, None)
+        pending, said, held = launch(order, None)
         while True:
             # the step after the one in flight, for the sequences that its token cannot end by count
             ahead = [i for i in order if i in slots and len(generated[i]) + 2 <= params.max_tokens
@@ -208,14 +251,15 @@ class Generator:
                 if saves:
                     saved = chooser.save_streams()
                 following = launch(ahead, chooser.rows_of(pending, rows))
-            take(order, chooser.read(pending), held)
+            tokens = chooser.read(pending)
+            take(order, tokens, held, logprobs.read(said, tokens) if logprobs is not None else None)
             if saved is not None:
                 for i in ahead:
                     if i not in slots and i in kept:        # it ended on this token: the draw after it never was
                         chooser.restore_stream(i, saved)
             if not live or following is None:
                 break
-            order, (pending, held) = ahead, following
+            order, (pending, said, held) = ahead, following
 
     def extend(self, slot, tokens, params, chooser, on_token=None, interrupt=None):
         """One more turn of a sequence whose slot the caller keeps (the reference's
@@ -227,6 +271,8 @@ class Generator:
         generator streams go on from turn to turn); sequence index 0 is used. Returns one
         GenerationResult."""
         params.validate()
+        if params.samples != 1:
+            raise RequestError("a turn has one answer")
         if not tokens:
             raise RequestError("a turn needs at least one token")
         eng = self.engine
@@ -246,13 +292,23 @@ class Generator:
         eng = self.engine
         eos = eng.spec.eos_token_id
         kept = kept or {}
-        slots = {i: kept[i] if i in kept else eng.alloc_slot() for i in members}
+        # answers to one prompt that stand side by side: the first one's slot takes the prompt, the others are forked from it
+        leader = {}
+        for at, i in enumerate(members):
+            same = params.samples > 1 and at > 0 and members[at - 1] // params.samples == i // params.samples
+            leader[i] = leader[members[at - 1]] if same else i
+        logprobs = None
+        if params.logprobs is not None:
+            from ..sampling.logprobs import LogprobReader
+            logprobs = LogprobReader(params.logprobs, eng.spec.vocab_size, eng.device)
+        slots = {}
         before = {i: eng.cache.length(kept[i]) for i in kept}
         generated = {i: [] for i in members}
+        said_of = {i: None if logprobs is None else [] for i in members}
         live = list(members)
 
         def finish(i, reason):
-            results[i] = GenerationResult(generated[i], reason, len(prompts[i]))
+            results[i] = GenerationResult(generated[i], reason, len(prompts[i]), said_of[i])
             slot = slots.pop(i)
             if i in kept:
                 # a step that ran ahead of the host has taken the newest token in already
@@ -262,17 +318,20 @@ class Generator:
             live.remove(i)
 
         try:
+            for i in members:
+                if leader[i] == i:
+                    slots[i] = kept[i] if i in kept else eng.alloc_slot()
             t0 = time.perf_counter()
-            tokens = self._prompts(live, prompts, slots, chooser)
+            tokens, said = self._prompts(live, prompts, slots, chooser, leader, logprobs)
             self.stats.prefill_seconds += time.perf_counter() - t0
-            self.stats.prompt_tokens += sum(len(prompts[i]) for i in live)
+            self.stats.prompt_tokens += sum(len(prompts[i]) for i in live if leader[i] == i)
             t0 = time.perf_counter()
 
-            def take(order, tokens, held=None):
+            def take(order, tokens, held=None, said=None):
                 """The newest tokens of the sequences `order` (those that have ended since are
                 skipped). `held`: the positions each sequence held when the step that chose these
                 tokens had been put on the stream, if a later step has been since."""
-                for i, tok in zip(order, tokens):
+                for at, (i, tok) in enumerate(zip(order, tokens)):
                     if i not in slots:
                         continue
                     if not 0 <= int(tok) < eng.spec.vocab_size:
@@ -281,11 +340,13 @@ class Generator:
                         raise BackendError(f"request {i}: no token could be chosen (got {int(tok)}): its logits "
                                            "hold no finite value")
                     generated[i].append(int(tok))
+                    if said is not None:
+                        said_of[i].append(said[at])
                     self.stats.generated_tokens += 1
-                    said = on_token(i, int(tok)) if on_token is not None else None
+                    answer = on_token(i, int(tok)) if on_token is not None else None
                     reason = stop_reason(generated[i], params, eos)
-                    if reason is None and isinstance(said, str):
-                        reason = said
+                    if reason is None and isinstance(answer, str):
+                        reason = answer
                     length = eng.cache.length(slots[i]) if held is None else held[i]
                     if reason is None and length >= eng.spec.max_positions:
                         reason = LENGTH
@@ -295,18 +356,19 @@ class Generator:
                     for i in list(live):
                         finish(i, INTERRUPTED)
 
-            take(list(live), tokens)
+            take(list(live), tokens, None, said)
             # (a kept slot is rolled back by the one step that ran ahead: only where the cache can)
             if self.run_ahead and getattr(chooser, "can_run_ahead", False) and \
                     getattr(eng, "accepts_device_tokens", False) and \
                     (not kept or getattr(eng.cache, "rolls_back_freely", False)):
-                self._decode_ahead(live, slots, generated, params, chooser, take, kept)
+                self._decode_ahead(live, slots, generated, params, chooser, take, kept, logprobs)
             else:
                 while live:
                     order = list(live)
                     logits = eng.step([StepEntry(slots[i], [generated[i][-1]], [0]) for i in order], **self._views)
                     self.stats.decode_steps += 1
-                    take(order, chooser.choose(logits, order))
+                    tokens, said = self._choose(chooser, logits, order, logprobs)
+                    take(order, tokens, None, said)
             self.stats.decode_seconds += time.perf_counter() - t0
         finally:
             for i in list(slots):

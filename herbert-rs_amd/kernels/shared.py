@@ -9,7 +9,7 @@ import numpy as np
 import torch
 
 from ..errors import BackendError
-from ..hosted import send
+from ..hosted import send, send_into
 from . import lib, mfma, ops
 from .ops import _check, _stream
 
@@ -23,6 +23,8 @@ COLUMNS = {torch.bfloat16: 128, torch.float32: 16}      # (row, head) pairs of a
 F32_MOST_DIM = 256
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
 FOUR_MOST_PAGES = 8
+SAVED_BYTES = 60 << 20
+MANY_TOKENS = 8
 
 
 def supported(kv, nq, nkv, hd, dtype):
@@ -34,7 +36,7 @@ def supported(kv, nq, nkv, hd, dtype):
     return dtype == torch.float32 and hd % 4 == 0 and 0 < hd <= F32_MOST_DIM
 
 
-def plan(starts, context, slots, sharing, group, nkv, columns, workgroups):
+def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=1):
     """How a step is cut up. starts: the first packed row of each sequence and the last one's end; context: the positions it
     holds after the step; slots: theirs; sharing: a SharedPages. Returns int32 arrays (items [n, 8], order [rows], part_start
     [rows + 1], parts) and the most rows of an item; see csrc/attention_shared.hip.
@@ -89,39 +91,109 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups):
     # the longest items first, those over the same pages side by side
     items = items[np.lexsort((items[:, 0], items[:, 3], items[:, 3] - items[:, 4]))]
     most = int(n.max())
+    single = heads = items[:0]
     if columns == 128 and len(items) * nkv > workgroups:
         # more workgroups than the GPU holds at a time: short items are a wave each
         short = (items[:, 1] * group <= 32) & (items[:, 4] - items[:, 3] <= FOUR_MOST_PAGES)
-        alone, single = items[~short], items[short]
+        items, single = items[~short], items[short]
         heads = np.zeros((-(-len(single) // 4), ITEM_INTS), dtype=np.int64)
-        n_items = len(alone) + len(heads)
+    n_items = -(-(len(items) + len(heads)) // grid) * grid
+    if len(heads):
         heads[:, 0] = n_items + 4 * np.arange(len(heads))
         heads[:, 1] = heads[:, 7] = 1
-        rest = np.zeros((4 * len(heads) - len(single), ITEM_INTS), dtype=np.int64)
-        items = np.concatenate([alone, heads, single, rest])
-    else:
-        n_items = len(items)
+    nothing = lambda count: np.zeros((count, ITEM_INTS), dtype=np.int64)
+    items = np.concatenate([items, heads, nothing(n_items - len(items) - len(heads)), single, nothing(4 * len(heads) - len(single))])
     as32 = lambda x: np.ascontiguousarray(x, dtype=np.int32)
     return as32(items), as32(order), as32(part_start), as32(parts), n_items, most
 
 
-class _Plan:
+def _planned(meta, group, nkv, dtype, grid=1):
+    return plan(meta.host_starts, meta.host_context, meta.host_slots, meta.shared, group, nkv, COLUMNS[dtype], WORKGROUPS[dtype], grid)
+
+
+class Plan:
     """A plan on the GPU."""
 
-    def __init__(self, arrays, n_items, max_rows, device):
-        items, order, part_start, parts = arrays
-        both = send(np.concatenate([a.ravel() for a in arrays]), device)
-        at = np.cumsum([a.size for a in arrays])
+    def __init__(self, meta, group, nkv, dtype):
+        items, order, part_start, parts, self.n_items, self.max_rows = _planned(meta, group, nkv, dtype)
+        both = send(np.concatenate([a.ravel() for a in (items, order, part_start, parts)]), meta.positions.device)
+        at = np.cumsum([a.size for a in (items, order, part_start, parts)])
         self.items, self.order, self.part_start, self.parts = both[:at[0]], both[at[0]:at[1]], both[at[1]:at[2]], both[at[2]:]
-        self.n_items, self.n_parts, self.max_rows = n_items, len(parts), max_rows
+        self.n_parts = len(parts)
 
 
-def _plan_of(meta, nq, nkv, dtype):
-    key = ("shared_plan", nq // nkv, nkv, dtype)
+class StaticPlan:
+    """The plans of decode steps of one batch size, in buffers that stay where they are while they are large enough: a recorded
+    graph reads them. `shape` is what such a graph is tied to: which buffers, how many workgroups (in steps of GRID) and how much room
+    for partial results (powers of two)."""
+    GRID = 16
+
+    def __init__(self, group, nkv, dtype, rows, device):
+        self.group, self.nkv, self.dtype, self.rows, self.device = group, nkv, dtype, rows, device
+        self.max_rows = max(1, COLUMNS[dtype] // group)
+        self.made = 0               # buffers so far: those that were outgrown are kept, a graph may hold their addresses
+        self._outgrown = []
+        self._buffer, self._rooms, self._filled_for = None, (0, 0), None
+        self.n_items = self.n_parts = 0
+
+    @property
+    def shape(self):
+        return self.made, self.n_items, self.n_parts
+
+    def refill(self, meta):
+        """Work the step's plan out and send it, unless it is that of the step before (it changes where a sequence begins a page)."""
+        filled_for = (meta.shared, meta.host_slots.tobytes(), ((meta.host_context - 1) // 64).tobytes())
+        before = self._filled_for
+        if before is not None and before[0] is meta.shared and before[1:] == filled_for[1:]:
+            return
+        items, order, part_start, parts, self.n_items, _ = _planned(meta, self.group, self.nkv, self.dtype, self.GRID)
+        self.n_parts = 1 << (len(parts) - 1).bit_length()
+        if len(items) > self._rooms[0] or len(parts) > self._rooms[1]:
+            if self._buffer is not None:
+                self._outgrown.append(self._buffer)
+            self._rooms = (2 * len(items), 2 * len(parts))
+            self._buffer = torch.zeros(ITEM_INTS * self._rooms[0] + 2 * self.rows + 1 + self._rooms[1], dtype=torch.int32, device=self.device)
+            self.made += 1
+        at = np.cumsum([ITEM_INTS * self._rooms[0], self.rows, self.rows + 1, self._rooms[1]])
+        b = self._buffer
+        self.items, self.order, self.part_start, self.parts = b[:at[0]], b[at[0]:at[1]], b[at[1]:at[2]], b[at[2]:]
+        host = np.zeros(at[2] + len(parts), dtype=np.int32)
+        host[:items.size], host[at[0]:at[1]], host[at[1]:at[2]], host[at[2]:] = items.ravel(), order, part_start, parts
+        send_into(host, b[:len(host)])
+        self._filled_for = filled_for
+
+
+def _saved(meta, nkv, hd, dtype):
+    return meta.shared.pages_saved * nkv * 64 * hd * 2 * (4 if dtype == torch.float32 else 2)
+
+
+def pays(meta, kv, nq, nkv, hd, dtype):
+    """True where the shared attention takes this step over this cache and ends sooner than the attention that reads every sequence's pages
+    by itself: by the bytes of keys and values that are not read again."""
+    return meta.shared is not None and supported(kv, nq, nkv, hd, dtype) and _ends_sooner(meta, nkv, hd, dtype)
+
+
+def _ends_sooner(meta, nkv, hd, dtype):
+    if meta.shared is None:
+        return False
+    if dtype == torch.float32:
+        return True
+    if meta.max_new > 1 and meta.num_tokens > MANY_TOKENS * meta.num_seqs:
+        return False
+    return _saved(meta, nkv, hd, dtype) >= SAVED_BYTES
+
+
+def _plan_of(meta, nq, nkv, hd, dtype):
+    key = ("shared_plan", nq // nkv, nkv, hd, dtype)
+    if meta.static is not None:
+        found = meta.static.shared_plan(key, lambda rows, device: StaticPlan(nq // nkv, nkv, dtype, rows, device),
+                                        lambda m: _ends_sooner(m, nkv, hd, dtype))
+        if found is None:
+            raise BackendError("shared attention: it does not pay for this step (see pays)")
+        return found
     found = meta.derived.get(key)          # every layer's attention asks: worked out once a step
     if found is None:
-        *arrays, n_items, max_rows = plan(meta.host_starts, meta.host_context, meta.host_slots, meta.shared, nq // nkv, nkv, COLUMNS[dtype], WORKGROUPS[dtype])
-        found = meta.derived[key] = _Plan(arrays, n_items, max_rows, meta.positions.device)
+        found = meta.derived[key] = Plan(meta, nq // nkv, nkv, dtype)
     return found
 
 
@@ -144,7 +216,7 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     _check(meta.positions, "positions", torch.int32, (T,))
     if sinks is not None:
         _check(sinks, "sinks", torch.float32, (nq,))
-    p = _plan_of(meta, nq, nkv, q.dtype)
+    p = _plan_of(meta, nq, nkv, hd, q.dtype)
     po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
     lib.call("attention_shared", "hb_attn_shared", q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), out.data_ptr(), ops.dtype_code(q),
              po.data_ptr(), pml.data_ptr(), p.items.data_ptr(), p.n_items, p.max_rows, p.order.data_ptr(), p.part_start.data_ptr(),

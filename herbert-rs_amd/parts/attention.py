@@ -35,6 +35,9 @@ attention itself (mfma.attention_decode_heads), the heads' difference, gate and 
 head are two query heads of one kept key, which holds both maps' keys side by side, with zeros in a query where
 the other map lies: the values are kept and read once.
 
+Where sequences of a step share pages (forked slots), either form without window, chunks and biases by distance reads
+those pages once for all of them where that ends sooner (kernels.shared), one map a head.
+
 Three further options go with either form (not in the reference): `keep_first` (with a window: the sequence's first
 so many keys are seen as well; the cache keeps their pages), `distance_bias=(bias_max,)` (a learned bias by the
 distance of query and key, a table [rows, heads] whose rows the stored tensor counts, is added to the scaled
@@ -53,7 +56,7 @@ import math
 import torch
 
 from ..cache import KVNeed, StateNeed
-from ..kernels import heads, mfma, ops, recurrent
+from ..kernels import heads, mfma, ops, recurrent, shared
 from ..weights import TensorNeed
 from .base import Part
 from .linear import Linear
@@ -313,8 +316,9 @@ class Attention(Part):
         angles, rot_dims, halves = self.position.step_angles(ctx) if hasattr(self.position, "step_angles") else (None, 0, False)
         gate_off = L.channels if self.gate else None
         plain_masks = not self.keep_first and self.distance_raw is None
-        fused = plain_masks and mfma.decode_heads_fusable(meta, kv, L, rt.dtype)
-        cores = plain_masks and mfma.heads_supported(kv, L, rt.dtype)
+        shares = self.maps == 1 and self._shares(ctx, kv)
+        fused = plain_masks and not shares and mfma.decode_heads_fusable(meta, kv, L, rt.dtype)
+        cores = plain_masks and not shares and mfma.heads_supported(kv, L, rt.dtype)
         # (slices of K are added up by the kernels that read the projection, but for the one that only gates heads)
         defer = rt.dtype == torch.bfloat16 and (self.hd == 128 if fused else L.adds_slices and self.proj_width % 4 == 0 and (
             cores or self.maps == 2 or not self.gate))
@@ -448,7 +452,7 @@ class Attention(Part):
         qkv = rt.buffer("qkv", (T, width), torch.float32)
         fused_decode = False
         if write_kv and rt.dtype == torch.bfloat16:
-            fused_decode = mfma.decode_fusable(ctx.meta, kv, self.nq, self.nkv, self.hd, rot_dims, rt.dtype)
+            fused_decode = not self._shares(ctx, kv) and mfma.decode_fusable(ctx.meta, kv, self.nq, self.nkv, self.hd, rot_dims, rt.dtype)
         slices = None
         if fused_norm is not None:
             self.qkv.forward_normed(x, fused_norm.w, fused_norm.eps, qkv)
@@ -474,8 +478,17 @@ class Attention(Part):
         self.attend(ctx, q, kv, attn)
         self.project_out(ctx, attn, x)
 
+    def _shares(self, ctx, kv):
+        """True where pages that several sequences of the step hold are read once for all of them."""
+        return (ctx.meta.shared is not None and not self.window and self.chunk is None and self.distance_raw is None
+                and shared.pays(ctx.meta, kv, self.kept_heads, self.nkv, self.hd, ctx.rt.dtype))
+
     def attend(self, ctx, q, kv, out):
         scale = self.scale if self.prepared else self.kernel_scale
+        if out.dtype == q.dtype and self._shares(ctx, kv):
+            shared.attention(q, ctx.meta, kv, out, self.kept_heads, self.nkv, self.hd, scale, sinks=self.sink_w, softcap=self.softcap,
+                             scratch=ctx.rt.scratch)
+            return
         if q.dtype == torch.bfloat16:
             if out.dtype == q.dtype and mfma.attention_supported(q, kv, self.kept_heads, self.nkv, self.hd):
                 mfma.attention(q, ctx.meta, kv, out, self.kept_heads, self.nkv, self.hd, scale, self.window,

@@ -3,13 +3,15 @@
 Names, meanings and defaults follow the reference's command line
 (crates/cli/src/main.rs:54-195): temperature 0.4 (0 = greedy), top_k 40
 (0 = off), top_p 0.9 (1.0 = off), max_tokens 2048, ignore_eos, no_repeat_check,
-think_budget 0 (no cap).
+think_budget 0 (no cap). The reference has neither `samples` nor `logprobs`.
 """
 from dataclasses import dataclass, field
 from typing import Optional, Tuple
 
 from ..errors import RequestError
 from .think import ThinkTokens
+
+MOST_ALTERNATIVES = 64          # a token (kernels.ops.LOGPROB_MOST)
 
 
 @dataclass(frozen=True)
@@ -24,6 +26,8 @@ class SamplingParams:
     seed: Optional[int] = None                      # None: from the clock, as the reference does
     think_budget: int = 0                           # most tokens inside a think block, 0 = no cap
     think_tokens: Optional[ThinkTokens] = None      # the ids that cap needs (sampling.think.ThinkTokens)
+    samples: int = 1                                # answers to every prompt, each with a generator stream of its own
+    logprobs: Optional[int] = None                  # every token's log probability, entropy and so many alternatives (None: not)
 
     def validate(self):
         if self.temperature < 0:
@@ -36,6 +40,10 @@ class SamplingParams:
             raise RequestError("max_tokens must be > 0")
         if self.think_budget < 0:
             raise RequestError("think_budget must be >= 0")
+        if self.samples < 1:
+            raise RequestError("samples must be >= 1")
+        if self.logprobs is not None and not 0 <= self.logprobs <= MOST_ALTERNATIVES:
+            raise RequestError(f"logprobs must be between 0 and {MOST_ALTERNATIVES} alternatives")
         if self.think_budget > 0 and self.think_tokens is None:
             raise RequestError("think_budget needs think_tokens (the ids that open and close a think block "
                                "and of a line break)")

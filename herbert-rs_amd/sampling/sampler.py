@@ -115,6 +115,11 @@ class Sampler:
                                           and vocab > ops.NUCLEUS_CANDIDATES)
 
     @property
+    def changes_logits(self):
+        """Whether `choose` may write into the logits (a think budget leaves a forced token as the only one)."""
+        return self.think is not None
+
+    @property
     def can_run_ahead(self):
         """Whether `choose_ahead` may be used: the tokens then stay on the GPU, where the next
         step can take them from, and the host reads them later."""

@@ -1,0 +1,288 @@
+"""Forked slots, several answers to a prompt, log probabilities and scoring through the engine."""
+import importlib
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import herbert_rs_amd as hb
+from herbert_rs_amd.engine import StepEntry
+from herbert_rs_amd.errors import CacheError, RequestError
+from herbert_rs_amd.kernels import shared
+
+from .bounds import BF16_REL_RMS, F32_ABS, close
+from .plain_cache import plain_logits
+from .tiny import CONFIGS, make_folder, random_tokens
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def used(monkeypatch):
+    """Shared pages are read together whatever they save (tiny models save little); counts the calls that do."""
+    calls = []
+    monkeypatch.setattr(shared, "SAVED_BYTES", 1)
+    monkeypatch.setattr(shared, "MANY_TOKENS", 1000)
+    real = shared.attention
+
+    def counted(*args, **kw):
+        calls.append(args[0].shape[0])
+        return real(*args, **kw)
+    monkeypatch.setattr(shared, "attention", counted)
+    return calls
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("name", ["B", "D", "C"])
+def test_forks_go_on_as_if_each_had_had_the_prompt(name, dtype, graphs, used, model_root):
+    """One prompt, five ways on, over page borders, with and without graphs; one of them ends early, one is rolled back and
+    goes another way, and the window of one configuration gives pages up."""
+    folder, vocab = make_folder(model_root, name, dtype), CONFIGS[name][0]["vocab_size"]
+    engine = hb.Engine.from_folder(folder, dtype=dtype, max_tokens=64 * 24, use_graphs=graphs)
+    prompt = random_tokens(vocab, 150, 1)
+    ways = [random_tokens(vocab, 75, 10 + i) for i in range(5)]
+    first = engine.alloc_slot()
+    engine.step([StepEntry(first, prompt, [149])])
+    slots = [first] + engine.fork(first, 4)
+    live = list(range(5))
+    for at in range(75):
+        if at == 30:
+            engine.free_slot(slots[2])
+            live.remove(2)
+        rows = engine.step([StepEntry(slots[i], [ways[i][at]], [0]) for i in live]).cpu().numpy()
+        if at % 6 == 0 or at > 66:
+            for i, row in zip(live, rows):
+                tokens = prompt + ways[i][:at + 1]
+                ok, err = close(row, plain_logits(folder, prompt + ways[i])[len(tokens) - 1], dtype, name, "forks")
+                assert ok, f"way {i}, position {len(tokens) - 1}: {err}"
+        engine.cache.check()
+    # (a graph's replay makes no calls; in bfloat16 heads of 48 go to kernels that read every sequence's pages by themselves)
+    assert len(used) > (3 if graphs else 70) or (name == "C" and dtype == "bfloat16")
+    if name != "C":                                     # (a window that has given keys up cannot be rolled back)
+        engine.truncate(slots[1], 160)
+        other = random_tokens(vocab, 9, 77)
+        rows = engine.step([StepEntry(slots[1], other, list(range(9))), StepEntry(slots[0], [3], [0])]).cpu().numpy()
+        ref = plain_logits(folder, prompt + ways[1][:10] + other)
+        for j in range(9):
+            assert close(rows[j], ref[160 + j], dtype, name, "forks")[0]
+        assert close(rows[9], plain_logits(folder, prompt + ways[0] + [3])[-1], dtype, name, "forks")[0]
+    for i in live:
+        engine.free_slot(slots[i])
+    engine.cache.check()
+    assert all(g.pages.held_count == 0 for g in engine.cache.kv_groups.values())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_trees_of_forks_beside_strangers(dtype, used, model_root):
+    """Forks of forks, a sequence that shares nothing, and batch sizes that are filled up with padding rows; steps of many tokens too."""
+    folder, vocab = make_folder(model_root, "D", dtype), CONFIGS["D"][0]["vocab_size"]
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 60)
+    texts = {}
+    root = engine.alloc_slot()
+    texts[root] = random_tokens(vocab, 200, 1)
+    stranger = engine.alloc_slot()
+    texts[stranger] = random_tokens(vocab, 90, 2)
+    engine.step([StepEntry(s, t, []) for s, t in texts.items()])
+    branches = [root] + engine.fork(root, 2)
+    for s in branches[1:]:
+        texts[s] = list(texts[root])
+    more = {s: random_tokens(vocab, 70 + 30 * i, 20 + i) for i, s in enumerate(branches)}
+    engine.step([StepEntry(s, t, [len(t) - 1]) for s, t in more.items()])
+    for s, t in more.items():
+        texts[s] = texts[s] + t
+    for s in list(branches):
+        for new in engine.fork(s, 3):
+            texts[new] = list(texts[s])
+    for step in range(8):
+        n = 1 if step % 3 else 5
+        new = {s: random_tokens(vocab, n + (s % 3 if n > 1 else 0), 1000 * step + s) for s in texts}
+        rows = engine.step([StepEntry(s, t, [len(t) - 1]) for s, t in new.items()]).cpu().numpy()
+        for (s, t), row in zip(new.items(), rows):
+            texts[s] = texts[s] + t
+            if step in (0, 4, 7):
+                ok, err = close(row, plain_logits(folder, texts[s])[-1], dtype, "D", "trees")
+                assert ok, f"step {step}, slot {s}: {err}"
+        engine.cache.check()
+    assert len(used) >= 2
+
+
+FAMILIES = [("vipalorn_tiny", "Q"), ("modasun_tiny", "P"), ("mefatar_tiny", "P"), ("bozasun_tiny", "P"), ("mutedra_tiny", "P"),
+            ("figalorn_tiny", "P")]
+
+
+@pytest.mark.parametrize("dtype, together", [("float32", False), ("float32", True), ("bfloat16", False)])
+@pytest.mark.parametrize("module, name", FAMILIES)
+def test_forks_of_every_family_hold_state_of_their_own(module, name, dtype, together, used, model_root, monkeypatch):
+    """Two forks and their source go three ways, and three slots go the same ways that have each had the prompt: the same bits where every
+    sequence's pages are read by themselves, sums in another order (bounds.py) where shared ones are read together. (In bfloat16 a rounding
+    may send a token to another expert: no bound for logits there.)"""
+    if not together:
+        monkeypatch.setattr(shared, "pays", lambda *args: False)
+    tiny = importlib.import_module("tests." + module)
+    folder = tiny.make_folder(model_root, name, dtype)
+    vocab = tiny.CONFIGS[name][0]["vocab"]
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 24)
+    prompt = random_tokens(vocab, 75, 1)
+    ways = [random_tokens(vocab, 12, 30 + i) for i in range(3)]
+    got = []
+    for forked in (True, False):
+        first = engine.alloc_slot()
+        engine.step([StepEntry(first, prompt, [])])
+        slots = [first] + (engine.fork(first, 2) if forked else [engine.alloc_slot(), engine.alloc_slot()])
+        if not forked:
+            for s in slots[1:]:
+                engine.step([StepEntry(s, prompt, [])])
+        got.append([engine.step([StepEntry(s, [w[at]], [0]) for s, w in zip(slots, ways)]).cpu() for at in range(12)])
+        for s in slots:
+            engine.free_slot(s)
+        engine.cache.check()
+    for at, (a, b) in enumerate(zip(*got)):
+        assert torch.equal(a, b) or (together and (a - b).abs().max() <= F32_ABS), f"token {at}: {(a - b).abs().max()}"
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("chunk", [None, 50])
+def test_samples_are_the_answers_of_as_many_prompts(dtype, chunk, used, model_root):
+    """Seeded answers to one prompt are those to the prompt said as often: the same generator streams, the same logits (in float32 to the
+    token; in bfloat16 the answers of one greedy stream may leave each other at a near tie)."""
+    folder, vocab = make_folder(model_root, "B", dtype), CONFIGS["B"][0]["vocab_size"]
+    prompts = [random_tokens(vocab, 130, 5), random_tokens(vocab, 20, 6)]
+    kw = dict(temperature=0.8, top_k=12, top_p=0.95, max_tokens=40, seed=11, ignore_eos=True, no_repeat_check=True)
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 60)
+    got = hb.generate(engine, prompts, samples=4, prefill_chunk=chunk, **kw)
+    want = hb.generate(engine, [p for p in prompts for _ in range(4)], prefill_chunk=chunk, **kw)
+    assert [len(a) for a in got] == [4, 4] and used
+    same = [a == b for a, b in zip([s for a in got for s in a], want)]
+    if dtype == "float32":
+        assert all(same)
+    else:
+        assert all(a[:3] == b[:3] for a, b in zip([s for a in got for s in a], want))
+    assert len({tuple(s) for s in got[0]}) > 1
+    engine.cache.check()
+    assert all(g.pages.held_count == 0 for g in engine.cache.kv_groups.values())
+    one = hb.generate(folder, prompts[0], samples=2, dtype=dtype, **dict(kw, max_tokens=3))
+    assert len(one) == 2 and all(len(s) == 3 for s in one)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kw", [dict(temperature=0.0), dict(temperature=0.9, top_k=20, seed=3), dict(temperature=0.9, top_k=0, top_p=0.9, seed=3)])
+def test_log_probabilities_of_generated_tokens(dtype, kw, model_root):
+    """Each generated token's log probability, entropy and alternatives are those of the logits that the engine gives for the same
+    positions, steps ahead of the host or not."""
+    folder, vocab = make_folder(model_root, "D", dtype), CONFIGS["D"][0]["vocab_size"]
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 20)
+    prompts = [random_tokens(vocab, 30, 5), random_tokens(vocab, 7, 6)]
+    params = hb.SamplingParams(max_tokens=12, ignore_eos=True, repeat_check=False, logprobs=4, samples=2, **kw)
+    results = engine.generate(prompts, params)
+    bare = engine.generate(prompts, hb.SamplingParams(max_tokens=12, ignore_eos=True, repeat_check=False, samples=2, **kw))
+    assert [r.tokens for r in results] == [r.tokens for r in bare] and bare[0].logprobs is None
+    for i, r in enumerate(results):
+        prompt = prompts[i // 2]
+        assert [t.token for t in r.logprobs] == r.tokens and len(r.tokens) == 12
+        slot = engine.alloc_slot()
+        logits = engine.step([StepEntry(slot, prompt + r.tokens[:-1], list(range(len(prompt) - 1, len(prompt) + 11)))]).double().cpu()
+        engine.free_slot(slot)
+        logp = torch.log_softmax(logits, -1)
+        entropy = -(logp.exp() * logp).sum(-1)
+        rms = logits.square().mean().sqrt().item()
+        # Two cuts of one text into steps: their logits are each within their bound (bounds.py) of the plain ones, so twice that
+        # apart; a log probability moves by up to twice as much, the entropy by sum p |log p + H| <= 2 H times as much.
+        apart = 2 * (F32_ABS if dtype == "float32" else BF16_REL_RMS["D"] * rms)
+        allowed = 2 * apart
+        for j, t in enumerate(r.logprobs):
+            assert abs(t.logprob - logp[j, t.token].item()) <= allowed
+            assert abs(t.entropy - entropy[j].item()) <= 2 * (entropy[j].item() + 1) * apart
+            assert len(t.top) == 4
+            for id_, lp in t.top:
+                assert abs(lp - logp[j, id_].item()) <= allowed
+            assert [lp for _, lp in t.top] == sorted((lp for _, lp in t.top), reverse=True)
+            assert t.top[0][1] >= logp[j].max().item() - allowed
+            if kw["temperature"] == 0.0:
+                assert t.top[0][0] == t.token and t.top[0][1] == t.logprob
+
+
+def test_log_probabilities_under_a_think_budget_are_the_model_s(model_root):
+    """Where a budget forces a token, its log probability is that of the logits before."""
+    folder, vocab = make_folder(model_root, "D", "float32"), CONFIGS["D"][0]["vocab_size"]
+    engine = hb.load(folder, dtype="float32", cache_tokens=64 * 20)
+    from herbert_rs_amd.sampling import ThinkTokens
+    think = ThinkTokens(open_id=5, close_id=6, newline_id=7)
+    prompt = random_tokens(vocab, 20, 8)
+    slot = engine.alloc_slot()
+    best = int(engine.step([StepEntry(slot, prompt, [19])]).argmax())
+    engine.free_slot(slot)
+    params = hb.SamplingParams(temperature=0.0, max_tokens=6, ignore_eos=True, repeat_check=False, logprobs=1, think_budget=1,
+                               think_tokens=ThinkTokens(open_id=best, close_id=6, newline_id=7))
+    r = engine.generate([prompt], params)[0]
+    assert 6 in r.tokens and think is not None
+    forced = next(t for t in r.logprobs if t.token == 6)
+    assert forced.logprob < -0.01 and forced.top[0][0] != 6
+    assert all(math.isfinite(t.logprob) for t in r.logprobs)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_scores_of_continuations(dtype, used, model_root, monkeypatch):
+    folder, vocab = make_folder(model_root, "D", dtype), CONFIGS["D"][0]["vocab_size"]
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 40)
+    prompt = random_tokens(vocab, 140, 3)
+    texts = [random_tokens(vocab, n, 40 + n) for n in (1, 9, 70, 3, 1, 25)]
+    want = []
+    for c in texts:
+        rows = torch.from_numpy(plain_logits(folder, prompt + c).astype(np.float64))[139:-1]
+        want.append((torch.log_softmax(rows, -1), rows.square().mean().sqrt().item()))
+    for slots, rows in ((None, 512), (3, 512), (None, 16)):
+        monkeypatch.setattr("herbert_rs_amd.engine.engine.SCORED_ROWS", rows)
+        if slots:
+            engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 40, max_slots=slots)
+        got = hb.score(engine, prompt, texts, top=3)
+        for c, said, (logp, rms) in zip(texts, got, want):
+            assert [t.token for t in said] == c
+            allowed = 2 * (F32_ABS if dtype == "float32" else BF16_REL_RMS["D"] * rms)      # (a log probability: twice its logits' bound)
+            for j, t in enumerate(said):
+                assert abs(t.logprob - logp[j, t.token].item()) <= allowed and len(t.top) == 3
+        engine.cache.check()
+        assert engine.cache.slots.held_count == 0
+    assert used
+    text = random_tokens(vocab, 50, 9)
+    alone = engine.score(text[:1], [text[1:]])[0]
+    raw = torch.from_numpy(plain_logits(folder, text).astype(np.float64))
+    ref, rms = torch.log_softmax(raw, -1), raw.square().mean(-1).sqrt()
+    for j, t in enumerate(alone):
+        allowed = 2 * (F32_ABS if dtype == "float32" else BF16_REL_RMS["D"] * rms[j].item())
+        assert t.top == [] and abs(t.logprob - ref[j, text[j + 1]].item()) <= allowed
+
+
+def test_what_scoring_and_forking_refuse(model_root):
+    engine = hb.load(make_folder(model_root, "B", "float32"), dtype="float32", cache_tokens=64 * 4, max_slots=2)
+    for bad in (([], [[1]]), ([1], []), ([1], [[]]), ([1], [[999]]), ([1], [[-1]]), ([1], [[True]]), ([1], [[1] * 300])):
+        with pytest.raises(RequestError):
+            engine.score(*bad)
+    with pytest.raises(RequestError):
+        engine.score([1], [[2]], top=65)
+    slot = engine.alloc_slot()
+    with pytest.raises(CacheError):
+        engine.fork(slot, 2)
+    with pytest.raises(CacheError):
+        engine.score([1], [[2, 3]])                    # one slot for the prompt and none for a continuation
+    engine.free_slot(slot)
+    engine.cache.check()
+    assert engine.cache.slots.held_count == 0
+
+
+def test_the_command_line_prints_samples_and_log_probabilities(model_root, capsys):
+    from herbert_rs_amd.cli import main
+    folder = make_folder(model_root, "B", "bfloat16")
+    args = ["--model", folder, "--prompt", "5,17,3", "--temperature", "0.7", "--seed", "3", "--max-tokens", "4", "--ignore-eos",
+            "--no-repeat-check"]
+    assert main(args + ["--samples", "3", "--logprobs", "2"]) == 0
+    out = capsys.readouterr().out
+    lines = out.splitlines()
+    assert [l for l in lines if l.startswith("---")] == ["--- 1 ---", "--- 2 ---", "--- 3 ---"]
+    ids = [l for l in lines if "," in l and "\t" not in l]
+    assert len(ids) == 3 and all(len(l.split(",")) == 5 for l in ids)
+    assert sum("\t" in l for l in lines) == 15
+    assert main(args + ["--logprobs", "0"]) == 0
+    assert sum("\t" in l for l in capsys.readouterr().out.splitlines()) == 5
+    assert main(args + ["--samples", "0"]) == 1
