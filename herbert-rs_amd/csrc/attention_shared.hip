@@ -19,13 +19,12 @@ HB_MODULE_ERROR_SLOT()
 
 // What an item says, 8 numbers each: its first row in the order of the rows, how many (0: nothing here), the slot whose
 // page table names its pages, its first page and the one behind its last, where its rows' places among the partial results are
-// listed, whether there is a place in its pages that one of its rows does not see, and whether it stands for four items, a wave each,
-// that lie from its first number on.
+// listed, whether there is a place in its pages that one of its rows does not see, and a number that is not used.
 #define ITEM_INTS 8
 struct Item {
-    int row0, rows, slot, page0, page1, list0, masked, four;
+    int row0, rows, slot, page0, page1, list0, masked;
     __device__ __forceinline__ explicit Item(const int* p)
-        : row0(p[0]), rows(p[1]), slot(p[2]), page0(p[3]), page1(p[4]), list0(p[5]), masked(p[6]), four(p[7]) {}
+        : row0(p[0]), rows(p[1]), slot(p[2]), page0(p[3]), page1(p[4]), list0(p[5]), masked(p[6]) {}
 };
 
 // ---------------------------------------------------------------- bfloat16
@@ -35,8 +34,8 @@ struct Item {
 // once for all four, the next page's scores on the matrix cores while this one's exponentials are worked out.
 // Narrow ones: operands stream from memory into registers, half a page at a time, in 16 x 16 x 32 products, whose operands are 64
 // neighbouring bytes of a row; a wave has 16 or 32 columns, the waves of a tile (four, or two each of two tiles) take the pages
-// in turn and add up their results through LDS. Short ones of up to 32 columns are a wave each, four to a workgroup. With more than 64
-// columns (a sequence's own rows over the pages that they see in part) a wave is a tile of 32 here, too.
+// in turn and add up their results through LDS. A sequence's own rows over the pages that they see in part (CAUSAL) are
+// narrow, too, in tiles of 16 columns.
 // 256 registers and 66 KB of LDS: two workgroups a CU, so that items that wait for memory and items that compute overlap.
 template <int HD>
 struct SharedSizes {
@@ -67,11 +66,11 @@ struct SharedArgs {
 // A narrow item's wave: NT tiles of 16 columns from column col0 on, every phases-th page of the item from the phase-th on. With more than one
 // phase all waves of the workgroup come here (there is a barrier).
 // An operand of half a page: keys (row 4 g + i of block b: key 8 g + 4 b + i, so that a lane's scores are 8 neighbouring keys), g = lane / 16.
-template <int HD, int NT>
+template <int HD, int NT, bool CAUSAL>
 __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it, const int* pt, int cols, int col0, int phase, int phases,
                                             int wave, int lane, char* lds) {
     constexpr int STEPS = HD / 32, BLOCKS = HD / 16, STAGE = PAGE * HD;
-    constexpr int DEPTH = NT == 1 ? 2 : 1;               // halves of a page in flight
+    constexpr int DEPTH = NT == 1 && !CAUSAL ? 2 : 1;    // halves of a page in flight
     const int c16 = lane & 15, g = lane >> 4;
     int token[NT], head[NT], place[NT], pos[NT];
     bool mine[NT];
@@ -117,23 +116,18 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
 #pragma unroll
         for (int s = 0; s < STEPS; ++s) qreg[t][s] = *(const bf16x8*)(qrow + s * 32);
     }
-    int seen_last = 0x7ffffffe, seen_by_all = 0x7ffffffe;
+    int seen_last = 0x7ffffffe;                           // what the last of the columns sees
     if (it.masked) {
         seen_last = -1;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             pos[t] = A.positions[token[t]];
             seen_last = max(seen_last, pos[t]);
-            seen_by_all = min(seen_by_all, pos[t]);
         }
 #pragma unroll
-        for (int off = 1; off < 16; off <<= 1) {
-            seen_last = max(seen_last, __shfl_xor(seen_last, off, 64));
-            seen_by_all = min(seen_by_all, __shfl_xor(seen_by_all, off, 64));
-        }
-        // (columns of one position: what the last of them does not see, no column sees, and the sums of all are spoiled alike)
-        if (seen_by_all == seen_last) seen_by_all = 0x7ffffffe;
+        for (int off = 1; off < 16; off <<= 1) seen_last = max(seen_last, __shfl_xor(seen_last, off, 64));
     }
+    uint32_t odd = 0;
     f32x4 oacc[NT][BLOCKS];
     float m[NT], l[NT];
 #pragma unroll
@@ -197,49 +191,23 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
         u32x4 keep;
 #pragma unroll
         for (int i = 0; i < 4; ++i) keep[i] = seen >= 2 * i + 2 ? 0xffffffffu : seen == 2 * i + 1 ? 0xffffu : 0u;
-        if (key0 + 31 <= seen_by_all) {
 #pragma unroll
-            for (int d = 0; d < BLOCKS; ++d) {
-                const bf16x8 clean = __builtin_bit_cast(bf16x8, __builtin_bit_cast(u32x4, v[d]) & keep);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, pb[t], oacc[t][d], 0, 0, 0);
-            }
-        } else {
-            // What is left that is not finite is taken out of the product, and the columns that see it get what their sums would
-            // be: a second product counts, for every entry and column, the keys whose value is +inf (1 each), -inf (128) or NaN
-            // (16384; of 32 keys no count runs into the next). (An exponent of ones: its lowest bit added carries into the
-            // sign's place; two numbers a word.)
-            bf16x8 sees[NT];
-#pragma unroll
-            for (int t = 0; t < NT; ++t)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) sees[t][e] = key0 + 8 * g + e <= pos[t] ? (__bf16)1.f : (__bf16)0.f;
-#pragma unroll
-            for (int d = 0; d < BLOCKS; ++d) {
-                u32x4 x = __builtin_bit_cast(u32x4, v[d]) & keep, kind;
+        for (int d = 0; d < BLOCKS; ++d) {
+            u32x4 x = __builtin_bit_cast(u32x4, v[d]) & keep;
+            if constexpr (CAUSAL) {
+                // A value without a size that only some of the columns see is taken out of the product; the rows are marked, and
+                // the kernel that joins looks for it. (An exponent of ones: its lowest bit added carries into the sign's
+                // place; two numbers a word.)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const uint32_t ones = (((x[i] & 0x7f807f80u) + 0x00800080u) >> 15) & 0x00010001u;
-                    const uint32_t nan = ones & (((x[i] & 0x007f007fu) + 0x007f007fu) >> 7);
-                    const uint32_t minus = ones & ~nan & (x[i] >> 15), plus = ones & ~nan & ~minus;
-                    kind[i] = nan * 0x4680u | minus * 0x4300u | plus * 0x3f80u;      // 16384, 128, 1
-                    x[i] &= ~(ones * 0xffffu);
+                    x[i] &= ~((ones << 16) - ones);
+                    odd |= ones;
                 }
-                const bf16x8 clean = __builtin_bit_cast(bf16x8, x);
-#pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    const f32x4 counts = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, kind), sees[t],
-                                                                                 f32x4{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
-                    oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, pb[t], oacc[t][d], 0, 0, 0);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int n = (int)counts[i];
-                        const bool plus = n & 127, minus = n & 0x3f80;
-                        oacc[t][d][i] += n >= 16384 || (plus && minus) ? __uint_as_float(0x7fc00000u) : plus ? INFINITY : minus ? -INFINITY : 0.f;
-                    }
-                }
-                __builtin_amdgcn_sched_barrier(0);
             }
+            const bf16x8 clean = __builtin_bit_cast(bf16x8, x);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, pb[t], oacc[t][d], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
         if (following < halves) load_values(following, v);
@@ -250,10 +218,12 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
         half(ka[0], va[0]);
         if constexpr (DEPTH == 2) half(ka[1], va[1]);
     }
+    const bool marked = CAUSAL && __builtin_amdgcn_ballot_w64(odd != 0) != 0;
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         l[t] += __shfl_xor(l[t], 16, 64);
         l[t] += __shfl_xor(l[t], 32, 64);
+        if (marked) l[t] = -l[t];                         // (a mark: sums are not below zero)
     }
     auto leave = [&](int t, int d) {
         if (mine[t]) *(f32x4*)(A.partial_o + ((size_t)place[t] * A.nq + head[t]) * HD + d * 16 + 4 * g) = oacc[t][d];
@@ -287,7 +257,13 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
 #pragma unroll
             for (int f = 0; f < PHASES; ++f) {
                 other[f].x = other[f].x == -INFINITY ? 0.f : fast_exp2((other[f].x - top) * A.c);
-                total = fmaf(other[f].x, other[f].y, total);
+                total = fmaf(other[f].x, CAUSAL ? fabsf(other[f].y) : other[f].y, total);
+            }
+            if constexpr (CAUSAL) {
+                bool some = false;
+#pragma unroll
+                for (int f = 0; f < PHASES; ++f) some |= __float_as_uint(other[f].y) >> 31;
+                total = some ? -total : total;
             }
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d) {
@@ -308,7 +284,7 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
     };
     if (phases == 4) {
         join(std::integral_constant<int, 4>{});
-    } else if (NT == 2 && phases == 2) {
+    } else if (phases == 2) {
         join(std::integral_constant<int, 2>{});
     } else {
 #pragma unroll
@@ -422,7 +398,8 @@ __device__ __forceinline__ void wide_item(const SharedArgs& A, const Item& it, c
             *(f32x4*)(po + d * 32 + 8 * qd + 4 * g2) = f32x4{oacc[d][4 * qd], oacc[d][4 * qd + 1], oacc[d][4 * qd + 2], oacc[d][4 * qd + 3]};
 }
 
-template <int HD>
+// CAUSAL: there are items of several columns that see different places.
+template <int HD, bool CAUSAL>
 __global__ void __launch_bounds__(256, 2)
 attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache,
                    float* __restrict__ partial_o, float* __restrict__ partial_ml, const int* __restrict__ items,
@@ -431,21 +408,21 @@ attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache,
     // (of the launch, not of the kernel: see the prompt kernels)
     extern __shared__ __attribute__((aligned(1024))) char shared_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    Item it(items + (size_t)(blockIdx.x / nkv) * ITEM_INTS);
-    const bool four = it.four;
-    if (four) it = Item(items + (size_t)(it.row0 + wave) * ITEM_INTS);
+    const Item it(items + (size_t)(blockIdx.x / nkv) * ITEM_INTS);
     if (it.rows == 0) return;
     const SharedArgs A = {q, k_cache, v_cache, partial_o, partial_ml, order, positions, parts, nq, nkv, (int)(blockIdx.x % nkv), nq / nkv, c, cap};
     const int cols = it.rows * A.G;
     const int* pt = page_table + (size_t)it.slot * max_pages;
-    if (cols > 64 && !it.masked) {
+    if (cols > 64) {
         wide_item<HD>(A, it, pt, cols, wave, lane, (bf16*)shared_lds);
         return;
     }
-    const int tiles = cols <= 32 ? 1 : cols <= 64 ? 2 : 4, phases = four ? 1 : 4 / tiles;
-    const int tile = four ? 0 : wave % tiles, phase = four ? 0 : wave / tiles;
-    if (cols <= 16) narrow_item<HD, 1>(A, it, pt, cols, 0, phase, phases, wave, lane, shared_lds);
-    else narrow_item<HD, 2>(A, it, pt, cols, tile * 32, phase, phases, wave, lane, shared_lds);
+    // (what is looked for in items of a sequence's own rows takes registers that a wave of 32 columns does not have)
+    const bool small = CAUSAL ? it.masked || cols <= 16 : cols <= 16;
+    const int tiles = small ? (cols <= 16 ? 1 : cols <= 32 ? 2 : 4) : cols <= 32 ? 1 : 2, phases = 4 / tiles;
+    const int tile = wave % tiles, phase = wave / tiles;
+    if (small) narrow_item<HD, 1, CAUSAL>(A, it, pt, cols, tile * 16, phase, phases, wave, lane, shared_lds);
+    else narrow_item<HD, 2, false>(A, it, pt, cols, tile * 32, phase, phases, wave, lane, shared_lds);
 }
 
 // ---------------------------------------------------------------- float32
@@ -628,127 +605,176 @@ attn_shared_f32_kernel(const float* __restrict__ q, const float* __restrict__ k_
 }
 
 // ---------------------------------------------------------------- joining
-// A wave a (token, query head): the partial results part_start[t] .. part_start[t + 1] - 1 of the t-th row, in their order. T: the type that
-// leaves; c: what a difference of references is multiplied by for a power of two (float32: natural units, expf). A chain of three waits:
-// where they lie, the results with their references, and the store.
-template <class T, int E>
+// Where the values that rows of one sequence see lie: for rows whose partial results are marked (a sum with a sign), because a value without a
+// size was taken out of a product (CAUSAL: there may be such).
+struct Spoiled {
+    const bf16* v_cache;
+    const int *positions, *seq_of, *slots, *page_table;
+    int max_pages, nkv;
+};
+
+// What the sum over all values that a row sees becomes if some of them have no size: entry d of a head.
+__device__ __forceinline__ float spoiled_sum(const Spoiled& s, float sum, int token, int kvh, int d, int hd) {
+    const int pos = s.positions[token];
+    const int* pt = s.page_table + (size_t)s.slots[s.seq_of[token]] * s.max_pages;
+    bool plus = false, minus = false, nan = false;
+#pragma unroll 1
+    for (int j = 0; j <= pos; ++j) {
+        const float v = hb_to_float(s.v_cache[(((size_t)pt[j / PAGE] * s.nkv + kvh) * hd + d) * PAGE + j % PAGE]);
+        plus |= v == INFINITY;
+        minus |= v == -INFINITY;
+        nan |= v != v;
+    }
+    if (nan || (plus && minus)) return __uint_as_float(0x7fc00000u);
+    return plus ? INFINITY : minus ? -INFINITY : sum;
+}
+
+// LANES lanes a (token, query head), four entries each: the partial results part_start[t] .. part_start[t + 1] - 1 of the t-th row, in their
+// order. T: the type that leaves; c: what a difference of references is multiplied by for a power of two (float32: natural units,
+// expf). A chain of three waits: where they lie, the results with their references, and the store.
+template <class T, int LANES, bool CAUSAL>
 __global__ void __launch_bounds__(256)
 attn_shared_join_kernel(const float* __restrict__ partial_o, const float* __restrict__ partial_ml, T* __restrict__ out,
                         const int* __restrict__ order, const int* __restrict__ part_start, int n_rows, int nq, int hd, float c,
-                        const float* __restrict__ sinks) {
+                        const float* __restrict__ sinks, Spoiled spoiled) {
     constexpr bool EXACT = sizeof(T) == 4;
     constexpr int AHEAD = 8;
-    const int lane = threadIdx.x & 63;
-    const int at = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int t = at / nq, h = at % nq;
-    if (t >= n_rows) return;
+    const int lane = threadIdx.x % LANES;
+    const int at = blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+    const bool exists = at < n_rows * nq;                 // (lanes of others go along: a wave's exchanges are among LANES)
+    const int t = exists ? at / nq : 0, h = exists ? at % nq : 0;
     const int first = part_start[t], n = part_start[t + 1] - first, row = order[t];
-    const float* const po = partial_o + ((size_t)first * nq + h) * hd + E * lane;
+    const bool there = 4 * lane < hd;
+    const float* const po = partial_o + ((size_t)first * nq + h) * hd + (there ? 4 * lane : 0);
     const float2* const ml = (const float2*)partial_ml + (size_t)first * nq + h;
     const size_t stride = (size_t)nq * hd;
-    const bool there = E * lane < hd;
-    float v[AHEAD][E];
+    f32x4 v[AHEAD];
     auto ask = [&](int s) {                               // (places beyond the last: the last, with a weight of 0)
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const float* p = po + (size_t)(s + u < n ? s + u : n - 1) * stride;
-#pragma unroll
-            for (int e = 0; e < E; ++e) v[u][e] = there ? p[e] : 0.f;
-        }
+        for (int u = 0; u < AHEAD; ++u) v[u] = *(const f32x4*)(po + (size_t)(s + u < n ? s + u : n - 1) * stride);
     };
     ask(0);
     auto weight = [&](float m, float top) { return m == -INFINITY ? 0.f : EXACT ? expf(m - top) : fast_exp2((m - top) * c); };
     float top = -INFINITY;
-    float2 kept = make_float2(-INFINITY, 0.f);            // this lane's, of the first 64
-    for (int s = lane; s < n; s += 64) {
+    float2 kept = make_float2(-INFINITY, 0.f);            // this lane's, of the first LANES
+    for (int s = lane; s < n; s += LANES) {
         const float2 x = ml[(size_t)s * nq];
         if (s == lane) kept = x;
         top = fmaxf(top, x.x);
     }
-    top = hb_wave_max(top);
-    float acc[E], total = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int s0 = 0; s0 < n; s0 += 64) {
+    for (int off = LANES / 2; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, LANES));
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+    float total = 0.f;
+    bool marked = false;
+    for (int s0 = 0; s0 < n; s0 += LANES) {
         if (s0 > 0) kept = s0 + lane < n ? ml[(size_t)(s0 + lane) * nq] : make_float2(-INFINITY, 0.f);
+        if constexpr (CAUSAL) {
+            marked |= kept.y < 0.f;
+            kept.y = fabsf(kept.y);
+        }
         const float w = weight(kept.x, top);
-        total += hb_wave_sum(w * kept.y);
-        const int here = n - s0 < 64 ? n - s0 : 64;
+        total = fmaf(w, kept.y, total);
+        const int here = n - s0 < LANES ? n - s0 : LANES;
         for (int s = 0; s < here; s += AHEAD) {
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
-                const float ws = __shfl(w, s + u < here ? s + u : 0, 64);
+                const float ws = __shfl(w, (s + u) % LANES, LANES);
+                const bool counts = s + u < here && ws != 0.f;
 #pragma unroll
-                for (int e = 0; e < E; ++e) acc[e] = s + u >= here || ws == 0.f ? acc[e] : fmaf(ws, v[u][e], acc[e]);
+                for (int e = 0; e < 4; ++e) acc[e] = counts ? fmaf(ws, v[u][e], acc[e]) : acc[e];
             }
             if (s0 + s + AHEAD < n) ask(s0 + s + AHEAD);
         }
     }
+#pragma unroll
+    for (int off = LANES / 2; off > 0; off >>= 1) {
+        total += __shfl_xor(total, off, LANES);
+        if (CAUSAL) marked |= __shfl_xor((int)marked, off, LANES) != 0;
+    }
     if (sinks) total += EXACT ? expf(sinks[h] - (top == -INFINITY ? 0.f : top)) : sink_share(sinks[h], top, c);
     const float inv = total > 0.f || total != total ? 1.0f / total : 0.f;
-    if (!there) return;
-    T* const dst = out + ((size_t)row * nq + h) * hd + E * lane;
+    if (!there || !exists) return;
+    if constexpr (CAUSAL) {
+        if (marked)
 #pragma unroll
-    for (int e = 0; e < E; ++e) dst[e] = hb_from_float<T>(acc[e] * inv);
+            for (int e = 0; e < 4; ++e) acc[e] = spoiled_sum(spoiled, acc[e], row, h / (nq / spoiled.nkv), 4 * lane + e, hd);
+    }
+    T* const dst = out + ((size_t)row * nq + h) * hd + 4 * lane;
+    if constexpr (EXACT) {
+        *(f32x4*)dst = acc * inv;
+    } else {
+        bf16x4 b;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) b[e] = (__bf16)(acc[e] * inv);
+        *(bf16x4*)dst = b;
+    }
 }
 
-// q, out [T, nq hd]; keys [pages, nkv, 64, hd], values [pages, nkv, hd, 64]; one storage type. items [n_items, 8] (and behind them those of
-// single waves); order [n_rows]; part_start [n_rows + 1]: where a row's partial results begin; parts: the places of the items' rows among
-// them; partial_o [partial results, nq, hd], partial_ml [partial results, nq, 2]. max_rows: the most rows of an item. softcap 0: none; sinks [nq] or null.
+// q, out [T, nq hd]; keys [pages, nkv, 64, hd], values [pages, nkv, hd, 64]; one storage type. items [n_items, 8]; order [n_rows]; part_start [n_rows + 1]: where a row's partial results begin; parts: the places of the items' rows among
+// them; partial_o [partial results, nq, hd], partial_ml [partial results, nq, 2]. max_rows: the most rows of an item;
+// causal: some rows are of one sequence (seq_of [n_rows], slots [sequences]: only then looked at). softcap 0: none; sinks [nq] or null.
 extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, float* partial_o,
-                              float* partial_ml, const int* items, int n_items, int max_rows, const int* order,
+                              float* partial_ml, const int* items, int n_items, int max_rows, int causal, const int* order,
                               const int* part_start, const int* parts, int n_rows, const int* positions,
-                              const int* page_table, int max_pages, int nq, int nkv, int hd, float scale, float softcap,
+                              const int* seq_of, const int* slots, const int* page_table, int max_pages, int nq, int nkv, int hd, float scale, float softcap,
                               const float* sinks, hipStream_t stream) {
     HB_REQUIRE(n_rows > 0 && n_items > 0 && nq > 0 && nkv > 0 && nq % nkv == 0, "shared attention: empty input, or heads that do not group");
     HB_REQUIRE(scale > 0.f && softcap >= 0.f, "shared attention: the scale must be positive, a cap of the scores too");
-    HB_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)partial_o) % 16 == 0,
+    HB_REQUIRE(((uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)partial_o | (uintptr_t)out) % 16 == 0,
                "shared attention: queries and pages lie on 16-byte borders");
     const int G = nq / nkv;
     const long long rows_of_heads = (long long)n_rows * nq;
-    HB_REQUIRE(rows_of_heads <= 0x7fffffffLL - 4, "shared attention: too many rows for the grid");
-    const dim3 join((unsigned)((rows_of_heads + 3) / 4));
+    HB_REQUIRE(rows_of_heads <= 0x7fffffffLL / 64, "shared attention: too many rows for the grid");
+    auto join = [&](int lanes) { return dim3((unsigned)((rows_of_heads * lanes + 255) / 256)); };
     if (dtype == HB_BF16) {
         HB_REQUIRE(hd == 32 || hd == 64 || hd == 128, "shared attention: bfloat16 heads of 32, 64 or 128, not %d", hd);
         HB_REQUIRE((long long)max_rows * G <= 128, "shared attention: items of %d rows x %d heads exceed 128 columns", max_rows, G);
         HB_REQUIRE((long long)n_items * nkv <= 0x7fffffffLL, "shared attention: too many items for the grid");
         const float c = scale * 1.4426950408889634f, cap = softcap > 0.f ? softcap / scale : 0.f;
+        const Spoiled spoiled = {(const bf16*)v_cache, positions, seq_of, slots, page_table, max_pages, nkv};
         const dim3 grid((unsigned)(n_items * nkv));
-#define HB_SHARED(HD, E)                                                                                                     \
+#define HB_SHARED_KERNEL(HD, CAUSAL)                                                                                       \
         {                                                                                                                    \
             constexpr int lds = SharedSizes<HD>::LDS;                                                                        \
-            static const hipError_t allowed =                                                                                \
-                hipFuncSetAttribute((const void*)attn_shared_kernel<HD>, hipFuncAttributeMaxDynamicSharedMemorySize, lds);   \
+            static const hipError_t allowed = hipFuncSetAttribute((const void*)attn_shared_kernel<HD, CAUSAL>,               \
+                                                                  hipFuncAttributeMaxDynamicSharedMemorySize, lds);          \
             HB_REQUIRE(allowed == hipSuccess, "shared attention: %d bytes of LDS refused: %s", lds, hipGetErrorString(allowed)); \
-            attn_shared_kernel<HD><<<grid, 256, lds, stream>>>((const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache,   \
-                                                               partial_o, partial_ml, items, order, parts, positions,        \
-                                                               page_table, max_pages, nq, nkv, c, cap);                      \
+            attn_shared_kernel<HD, CAUSAL><<<grid, 256, lds, stream>>>(                                                      \
+                (const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, partial_o, partial_ml, items, order, parts, positions, \
+                page_table, max_pages, nq, nkv, c, cap);                                                                     \
             HB_CHECK_LAUNCH("shared attention");                                                                             \
-            attn_shared_join_kernel<bf16, E><<<join, 256, 0, stream>>>(partial_o, partial_ml, (bf16*)out, order, part_start, \
-                                                                       n_rows, nq, hd, c, sinks);                            \
+            attn_shared_join_kernel<bf16, HD / 4, CAUSAL><<<join(HD / 4), 256, 0, stream>>>(partial_o, partial_ml, (bf16*)out, order,     \
+                                                                               part_start, n_rows, nq, hd, c, sinks, spoiled); \
         }
-        if (hd == 32) HB_SHARED(32, 1)
-        else if (hd == 64) HB_SHARED(64, 1)
-        else HB_SHARED(128, 2)
+#define HB_SHARED(HD)                                                                                                        \
+        {                                                                                                                    \
+            if (causal) HB_SHARED_KERNEL(HD, true)                                                                        \
+            else HB_SHARED_KERNEL(HD, false)                                                                              \
+        }
+        if (hd == 32) HB_SHARED(32)
+        else if (hd == 64) HB_SHARED(64)
+        else HB_SHARED(128)
 #undef HB_SHARED
+#undef HB_SHARED_KERNEL
     } else if (dtype == HB_F32) {
         HB_REQUIRE(hd > 0 && hd <= 256 && hd % 4 == 0, "shared attention: float32 heads of up to 256 entries in whole quads, not %d", hd);
         const long long col_tiles = ((long long)max_rows * G + 15) / 16;
         HB_REQUIRE((long long)n_items * nkv * col_tiles <= 0x7fffffffLL, "shared attention: too many items for the grid");
         const dim3 grid((unsigned)(n_items * nkv * col_tiles));
-#define HB_SHARED(NB, E)                                                                                                       \
+#define HB_SHARED(NB, LANES)                                                                                                      \
         {                                                                                                                      \
             attn_shared_f32_kernel<NB><<<grid, 256, 0, stream>>>((const float*)q, (const float*)k_cache, (const float*)v_cache, \
                                                                  partial_o, partial_ml, items, order, parts, positions,        \
                                                                  page_table, max_pages, nq, nkv, hd, scale, softcap,           \
                                                                  (int)col_tiles);                                              \
             HB_CHECK_LAUNCH("shared attention");                                                                               \
-            attn_shared_join_kernel<float, E><<<join, 256, 0, stream>>>(partial_o, partial_ml, (float*)out, order, part_start, \
-                                                                        n_rows, nq, hd, 0.f, sinks);                    \
+            attn_shared_join_kernel<float, LANES, false><<<join(LANES), 256, 0, stream>>>(partial_o, partial_ml, (float*)out, order, part_start, \
+                                                                        n_rows, nq, hd, 0.f, sinks, Spoiled{});                    \
         }
-        if (hd <= 64) HB_SHARED(1, 1)
-        else if (hd <= 128) HB_SHARED(2, 2)
-        else HB_SHARED(4, 4)
+        if (hd <= 64) HB_SHARED(1, 16)
+        else if (hd <= 128) HB_SHARED(2, 32)
+        else HB_SHARED(4, 64)
 #undef HB_SHARED
     } else {
         HB_REQUIRE(false, "shared attention: unknown dtype %d", dtype);

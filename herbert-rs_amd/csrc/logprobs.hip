@@ -35,13 +35,15 @@ __device__ __forceinline__ float value_of(uint64_t key) {
     return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
 
-// e^u for u <= 0 by the hardware's power of two; the rounding of u log2 e, which grows with |u|, is put back.
+// e^u for u from -150 (e^-150 is 0 in 32 bits) to 0 by the hardware's power of two; the rounding of u log2 e, which grows with |u|, is
+// put back.
 __device__ __forceinline__ float exp_of(float u) {
     const float t = u * 1.44269502f;
-    const float left = fmaf(u, 1.44269502f, -t) + u * 1.92596303e-8f;
+    const float left = fmaf(u, 1.92596303e-8f, fmaf(u, 1.44269502f, -t));
     const float e = __builtin_amdgcn_exp2f(t);
-    return u > -150.f ? fmaf(e * left, 0.693147182f, e) : e;
+    return fmaf(e * left, 0.693147182f, e);
 }
+__device__ __forceinline__ float at_least_nothing(float u) { return u < -150.f ? -150.f : u; }      // (a NaN stays one)
 
 __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int off) {
     const uint32_t lo = __shfl_xor((int)(uint32_t)v, off, 64), hi = __shfl_xor((int)(uint32_t)(v >> 32), off, 64);
@@ -50,17 +52,17 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int off) {
 
 struct Selecting {
     uint64_t list[LISTED];
-    uint64_t groups[64], bound, wave_best[THREADS / 64];
-    int count;
+    uint64_t groups[64], wave_best[THREADS / 64];
+    int above[THREADS / 64][64], count;
 };
 
-// The `top` largest of the keys that `each(f)` hands to f one after the other (as the thread's own, key by key), written by
-// put(rank, key): ranks 0 .. top - 1, those that there is no key for with the key 0. largest: the thread's own largest key.
+// The `top` largest of the keys that a workgroup holds, written by put(rank, key): ranks 0 .. top - 1, those that there is no key
+// for with the key 0. largest: the thread's own largest key; each(bound, f) hands f the thread's keys from bound on, and may hand it others.
 // The n-th largest of the 64 largest keys of four threads each bounds the n largest of all from below, and few keys lie at or above it: those
 // are listed and ranked by counting. Where more are than the list holds, the largest is looked for `top` times.
 template <class Each, class Put>
 __device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, Put put) {
-    const int tid = threadIdx.x, lane = tid & 63;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t g = largest;
 #pragma unroll
     for (int off = 1; off <= 2; off <<= 1) {
@@ -68,17 +70,19 @@ __device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, 
         g = o > g ? o : g;
     }
     if ((tid & 3) == 0) sh.groups[tid >> 2] = g;
-    if (tid == 0) sh.count = 0, sh.bound = 0;
+    if (tid == 0) sh.count = 0;
     __syncthreads();
-    if (tid < 64) {
-        const uint64_t mine = sh.groups[lane];
-        int above = 0;
-        for (int i = 0; i < 64; ++i) above += sh.groups[i] > mine ? 1 : 0;
-        if (above == top - 1 && mine != 0) sh.bound = mine;        // (keys are of different ids, only 0 may be there twice)
-    }
+    const uint64_t of_lane = sh.groups[lane];             // (a wave counts a quarter of the groups that lie above)
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) above += sh.groups[16 * wave + i] > of_lane ? 1 : 0;
+    sh.above[wave][lane] = above;
     __syncthreads();
-    const uint64_t bound = sh.bound > 1 ? sh.bound : 1;
-    each([&](uint64_t key) {
+    above = (sh.above[0][lane] + sh.above[1][lane]) + (sh.above[2][lane] + sh.above[3][lane]);
+    // (keys are of different ids, only 0 may be there twice: no group has the n-th place, and every key counts)
+    const uint64_t found = __builtin_amdgcn_ballot_w64(above == top - 1 && of_lane != 0);
+    const uint64_t bound = found ? sh.groups[__ffsll((unsigned long long)found) - 1] : 1;
+    each(bound, [&](uint64_t key) {
         if (key >= bound) {
             const int at = atomicAdd(&sh.count, 1);
             if (at < LISTED) sh.list[at] = key;
@@ -90,6 +94,7 @@ __device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, 
         for (int i = tid; i < count; i += THREADS) {
             const uint64_t mine = sh.list[i];
             int above = 0;
+#pragma unroll 8
             for (int j = 0; j < count; ++j) above += sh.list[j] > mine ? 1 : 0;
             if (above < top) put(above, mine);
         }
@@ -99,13 +104,13 @@ __device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, 
     uint64_t before = ~(uint64_t)0;
     for (int n = 0; n < top; ++n) {
         uint64_t best = 0;
-        each([&](uint64_t key) { best = key < before && key > best ? key : best; });
+        each(1, [&](uint64_t key) { best = key < before && key > best ? key : best; });
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
             const uint64_t o = shfl_xor_u64(best, off);
             best = o > best ? o : best;
         }
-        if (lane == 0) sh.wave_best[tid >> 6] = best;
+        if (lane == 0) sh.wave_best[wave] = best;
         __syncthreads();
         best = sh.wave_best[0];
         for (int w = 1; w < THREADS / 64; ++w) best = sh.wave_best[w] > best ? sh.wave_best[w] : best;
@@ -163,27 +168,30 @@ logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restr
             for (int e = 0; e < 4; ++e) x[4 * j + e] = at + e < len ? row[first + at + e] : -INFINITY;
         }
     }
-    float m = -INFINITY;
-    bool nan = false;
+    float mine = x[0];
+    int which = 0;
 #pragma unroll
-    for (int i = 0; i < PER; ++i) {
-        m = fmaxf(m, x[i]);
-        nan |= x[i] != x[i];
+    for (int i = 1; i < PER; ++i) {
+        const bool more = x[i] > mine;
+        mine = more ? x[i] : mine;
+        which = more ? i : which;
     }
-    m = hb_wave_max(m);
+    float m = hb_wave_max(fmaxf(mine, -INFINITY));        // (of what is a number)
     if (lane == 0) red[0][wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    float S = 0.f, T = 0.f;
+    float S = 0.f, T = 0.f;                               // (a NaN ends up in S)
     if (m != -INFINITY) {
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const float u = x[i] - m, e = exp_of(u);
+            const float u = at_least_nothing(x[i] - m), e = exp_of(u);
             S += e;
-            T += e > 0.f ? e * u : 0.f;
+            T = fmaf(e, u, T);
         }
+    } else {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) S = x[i] != x[i] ? x[i] : S;
     }
-    if (nan) S = __uint_as_float(0x7fc00000u);
     S = hb_wave_sum(S);
     T = hb_wave_sum(T);
     if (lane == 0) red[1][wave] = S, red[2][wave] = T;
@@ -196,19 +204,13 @@ logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restr
         else leave_token(whole, S, T, row, V, tokens[r], chosen + r, entropy + r);
     }
     if constexpr (TOP) {
-        auto key_at = [&](int i) {
-            const int at = ((i >> 2) * THREADS + tid) * 4 + (i & 3);
-            return at < len ? key_of(x[i], first + at) : (uint64_t)0;
-        };
-        uint64_t largest = 0;
+        auto id_at = [&](int i) { return ((i >> 2) * THREADS + tid) * 4 + (i & 3); };
+        const uint64_t largest = id_at(which) < len ? key_of(mine, first + id_at(which)) : (uint64_t)0;
+        select_top(sh, top, largest, [&](uint64_t bound, auto f) {
+            const float least = bound > 1 ? value_of(bound) : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            const uint64_t k = key_at(i);
-            largest = k > largest ? k : largest;
-        }
-        select_top(sh, top, largest, [&](auto f) {
-#pragma unroll
-            for (int i = 0; i < PER; ++i) f(key_at(i));
+            for (int i = 0; i < PER; ++i)
+                if (x[i] >= least) f(id_at(i) < len ? key_of(x[i], first + id_at(i)) : (uint64_t)0);
         }, [&](int rank, uint64_t key) {
             if (chunks > 1) keys[(r * chunks + chunk) * top + rank] = key;
             else leave_top(whole, key, ids + r * top + rank, best + r * top + rank);
@@ -240,9 +242,9 @@ logprob_row_kernel(const float* __restrict__ logits, int V, const int* __restric
             S += s.y;                      // nothing, or NaN
             continue;
         }
-        const float down = s.x - m, e = exp_of(down);
+        const float down = at_least_nothing(s.x - m), e = exp_of(down);
         S = fmaf(e, s.y, S);
-        if (e > 0.f) T = fmaf(e, fmaf(down, s.y, s.z), T);
+        T = fmaf(e, fmaf(down, s.y, s.z), T);
     }
     S = hb_wave_sum(S);
     T = hb_wave_sum(T);
@@ -257,7 +259,7 @@ logprob_row_kernel(const float* __restrict__ logits, int V, const int* __restric
         const int n = chunks * top;
         uint64_t largest = 0;
         for (int i = tid; i < n; i += THREADS) largest = keys[i] > largest ? keys[i] : largest;
-        select_top(sh, top, largest, [&](auto f) {
+        select_top(sh, top, largest, [&](uint64_t, auto f) {
             for (int i = tid; i < n; i += THREADS) f(keys[i]);
         }, [&](int rank, uint64_t key) { leave_top(whole, key, ids + r * top + rank, best + r * top + rank); });
     }

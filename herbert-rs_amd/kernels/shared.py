@@ -15,14 +15,14 @@ from .ops import _check, _stream
 
 _P, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 lib.register_signatures("attention_shared", {
-    "hb_attn_shared": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P],
+    "hb_attn_shared": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P],
 })
 
 ITEM_INTS = 8
 COLUMNS = {torch.bfloat16: 128, torch.float32: 16}      # (row, head) pairs of a kv head that an item holds at most
 F32_MOST_DIM = 256
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
-FOUR_MOST_PAGES = 8
+MASKED_COLUMNS = 64          # of an item in whose pages are places that some of its rows see and others do not
 SAVED_BYTES = 60 << 20
 MANY_TOKENS = 8
 
@@ -34,6 +34,13 @@ def supported(kv, nq, nkv, hd, dtype):
     if dtype == torch.bfloat16:
         return hd in mfma.ATTENTION_HEAD_DIMS and nq // nkv <= 32
     return dtype == torch.float32 and hd % 4 == 0 and 0 < hd <= F32_MOST_DIM
+
+
+def _even(first, end, most):
+    """Cut first .. end into as few stretches of at most `most` as there can be, alike in length: (first, length)."""
+    count = -(-(end - first) // most)
+    cuts = [first + (end - first) * i // count for i in range(count + 1)]
+    return [(a, b - a) for a, b in zip(cuts[:-1], cuts[1:])]
 
 
 def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=1):
@@ -49,22 +56,22 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
     row_of = np.concatenate([[0], np.cumsum(counts[sharing.order])])            # a sequence's first row in the order
     order = np.concatenate([np.arange(starts[i], starts[i + 1]) for i in sharing.order])
     tall = max(1, columns // group)
+    short = max(1, MASKED_COLUMNS // group) if columns == 128 else tall
     tiles = []                                                                  # row0, rows, sequence, first page, end, first page seen in part
     for first, count, page, end in sharing.nodes:
         a, b, seq = int(row_of[first]), int(row_of[first + count]), int(sharing.order[first])
-        for r in range(a, b, tall):
-            n = min(tall, b - r)
+        for r, n in _even(a, b, tall):
             if end >= 0:
                 tiles.append((r, n, seq, page, end, end))
                 continue
-            # a tile of a sequence's own rows ends at the page of its last row; all of it is seen by all before the first row's page
-            whole, last = (int(context[seq]) - (b - r)) // 64, (int(context[seq]) - (b - (r + n)) - 1) // 64 + 1
+            # A sequence's own rows: all of them see what lies before the first row's page; a tile ends at the page of its last row.
+            whole, page_from = (int(context[seq]) - (b - r)) // 64, page
             if n * group > 64 and whole > page:
                 tiles.append((r, n, seq, page, whole, whole))
                 page_from = whole
-            else:
-                page_from = page
-            tiles.append((r, n, seq, page_from, last, whole))
+            for u, m in _even(r, r + n, short):
+                first_seen, last_seen = int(context[seq]) - (b - u), int(context[seq]) - (b - (u + m)) - 1
+                tiles.append((u, m, seq, page_from, last_seen // 64 + 1, first_seen // 64))
     row0, rows, seq, page, end, whole = np.array(tiles, dtype=np.int64).T
     cols, pages = rows * group, end - page
     turns = np.where(cols <= 32, 4, np.where(cols <= 64, 2, 1)) if columns == 128 else np.ones_like(cols)
@@ -91,20 +98,10 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
     # the longest items first, those over the same pages side by side
     items = items[np.lexsort((items[:, 0], items[:, 3], items[:, 3] - items[:, 4]))]
     most = int(n.max())
-    single = heads = items[:0]
-    if columns == 128 and len(items) * nkv > workgroups:
-        # more workgroups than the GPU holds at a time: short items are a wave each
-        short = (items[:, 1] * group <= 32) & (items[:, 4] - items[:, 3] <= FOUR_MOST_PAGES)
-        items, single = items[~short], items[short]
-        heads = np.zeros((-(-len(single) // 4), ITEM_INTS), dtype=np.int64)
-    n_items = -(-(len(items) + len(heads)) // grid) * grid
-    if len(heads):
-        heads[:, 0] = n_items + 4 * np.arange(len(heads))
-        heads[:, 1] = heads[:, 7] = 1
-    nothing = lambda count: np.zeros((count, ITEM_INTS), dtype=np.int64)
-    items = np.concatenate([items, heads, nothing(n_items - len(items) - len(heads)), single, nothing(4 * len(heads) - len(single))])
+    n_items = -(-len(items) // grid) * grid
+    items = np.concatenate([items, np.zeros((n_items - len(items), ITEM_INTS), dtype=np.int64)])
     as32 = lambda x: np.ascontiguousarray(x, dtype=np.int32)
-    return as32(items), as32(order), as32(part_start), as32(parts), n_items, most
+    return as32(items), as32(order), as32(part_start), as32(parts), most
 
 
 def _planned(meta, group, nkv, dtype, grid=1):
@@ -115,11 +112,11 @@ class Plan:
     """A plan on the GPU."""
 
     def __init__(self, meta, group, nkv, dtype):
-        items, order, part_start, parts, self.n_items, self.max_rows = _planned(meta, group, nkv, dtype)
+        items, order, part_start, parts, self.max_rows = _planned(meta, group, nkv, dtype)
         both = send(np.concatenate([a.ravel() for a in (items, order, part_start, parts)]), meta.positions.device)
         at = np.cumsum([a.size for a in (items, order, part_start, parts)])
         self.items, self.order, self.part_start, self.parts = both[:at[0]], both[at[0]:at[1]], both[at[1]:at[2]], both[at[2]:]
-        self.n_parts = len(parts)
+        self.n_items, self.n_parts = len(items), len(parts)
 
 
 class StaticPlan:
@@ -146,8 +143,8 @@ class StaticPlan:
         before = self._filled_for
         if before is not None and before[0] is meta.shared and before[1:] == filled_for[1:]:
             return
-        items, order, part_start, parts, self.n_items, _ = _planned(meta, self.group, self.nkv, self.dtype, self.GRID)
-        self.n_parts = 1 << (len(parts) - 1).bit_length()
+        items, order, part_start, parts, _ = _planned(meta, self.group, self.nkv, self.dtype, self.GRID)
+        self.n_items, self.n_parts = len(items), 1 << (len(parts) - 1).bit_length()
         if len(items) > self._rooms[0] or len(parts) > self._rooms[1]:
             if self._buffer is not None:
                 self._outgrown.append(self._buffer)
@@ -214,12 +211,14 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     _check(kv.v, "value pages", kv.k.dtype, (pages, nkv, hd, 64))
     _check(kv.page_table, "page_table", torch.int32, (None, None))
     _check(meta.positions, "positions", torch.int32, (T,))
+    _check(meta.seq_of, "seq_of", torch.int32, (T,))
+    _check(meta.slots, "slots", torch.int32, (meta.num_seqs,))
     if sinks is not None:
         _check(sinks, "sinks", torch.float32, (nq,))
     p = _plan_of(meta, nq, nkv, hd, q.dtype)
     po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
     lib.call("attention_shared", "hb_attn_shared", q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), out.data_ptr(), ops.dtype_code(q),
-             po.data_ptr(), pml.data_ptr(), p.items.data_ptr(), p.n_items, p.max_rows, p.order.data_ptr(), p.part_start.data_ptr(),
-             p.parts.data_ptr(), T, meta.positions.data_ptr(), kv.page_table.data_ptr(),
+             po.data_ptr(), pml.data_ptr(), p.items.data_ptr(), p.n_items, p.max_rows, 1 if meta.max_new > 1 else 0, p.order.data_ptr(), p.part_start.data_ptr(),
+             p.parts.data_ptr(), T, meta.positions.data_ptr(), meta.seq_of.data_ptr(), meta.slots.data_ptr(), kv.page_table.data_ptr(),
              kv.page_table.shape[1], nq, nkv, hd, float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
              _stream())

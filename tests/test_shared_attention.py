@@ -99,11 +99,8 @@ def test_items_cover_what_every_row_sees_once(seed):
     starts = np.concatenate([[0], np.cumsum(news)])
     context = [h + n for h, n in zip(held, news)]
     for columns, group, nkv in ((128, 4, 8), (128, 1, 2), (128, 32, 1), (128, 7, 4), (16, 2, 4), (16, 16, 1), (16, 24, 2)):
-        items, order, part_start, parts, n_items, most = shared.plan(starts, context, np.arange(len(held))[::-1], found, group, nkv, columns, 512)
-        fours = items[:n_items][items[:n_items, 7] == 1]                # (each stands for four that lie behind)
-        assert sorted(i for f in fours[:, 0] for i in range(f, f + 4)) == list(range(n_items, len(items)))
-        assert not items[n_items:, 7].any() and (items[n_items:, 1] * group <= 32).all()
-        items = np.concatenate([items[:n_items][items[:n_items, 7] == 0], items[n_items:]])
+        items, order, part_start, parts, most = shared.plan(starts, context, np.arange(len(held))[::-1], found, group, nkv, columns, 512)
+        assert columns == 16 or not items[items[:, 1] * group > max(64, group), 6].any()        # (only narrow items look at a mask)
         items = items[items[:, 1] > 0]
         assert sorted(order.tolist()) == list(range(starts[-1]))
         assert most == items[:, 1].max() and (most * group <= columns or (most == 1 and columns == 16))
@@ -152,8 +149,8 @@ def test_what_the_shared_attention_refuses():
 
 
 def call(**changed):
-    args = dict(q=None, k=None, v=None, out=None, dtype=1, po=None, pml=None, items=None, n_items=1, max_rows=1, order=None, start=None,
-                parts=None, n_rows=1, positions=None, table=None, max_pages=1, nq=4, nkv=2, hd=64, scale=0.1, softcap=0.0,
+    args = dict(q=None, k=None, v=None, out=None, dtype=1, po=None, pml=None, items=None, n_items=1, max_rows=1, causal=0, order=None, start=None,
+                parts=None, n_rows=1, positions=None, seq_of=None, slots=None, table=None, max_pages=1, nq=4, nkv=2, hd=64, scale=0.1, softcap=0.0,
                 sinks=None, stream=None)
     args.update(changed)
     lib.call("attention_shared", "hb_attn_shared", *args.values())
