@@ -21,9 +21,21 @@ lib.register_signatures("attention_shared", {
 ITEM_INTS = 8
 COLUMNS = {torch.bfloat16: 128, torch.float32: 16}      # (row, head) pairs of a kv head that an item holds at most
 F32_MOST_DIM = 256
+# Workgroups that a step is cut into: as many as the GPU holds at a time, two a CU in bfloat16, four in float32. Measured with 256, 384 and 512 in
+# bfloat16: 128 answers to 32,768 tokens 110, 95 and 89 us, 64 to 8,192 37, 33 and 33 us, 12 continuations of a text of 2,000 tokens
+# 46, 44 and 46 us.
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
-MASKED_COLUMNS = 64          # of an item in whose pages are places that some of its rows see and others do not
-SAVED_BYTES = 60 << 20
+MASKED_COLUMNS = 64             # of an item in whose pages are places that some of its rows see and others do not: the wide ones ask no mask
+# The attention of one sequence after another also normalizes, rotates and writes what the projection gave; before the shared one that is a kernel of its
+# own. Bytes that need not be read again from which the shared one ends sooner all the same, in a model's decode steps (36 layers of 32 heads of
+# 128 over 8; microseconds a layer, shared less separate): 2 answers to 8,192 and 16,384 tokens (34, 67 MB) +2.1, -3.8; 4 to 2,048 and
+# 4,096 (25, 50 MB) +1.0, -0.8; 8 to 1,024 and 2,048 (29, 59 MB) +4.3, +0.8; 16 to 1,024, 2,048 and 2,560 (63, 126, 157 MB) +6.1, +0.5, -2.4; 32
+# to 1,024 and 2,048 (130, 260 MB) +4.3, -5.2; 64 to 1,024 and 2,048 (264, 528 MB) -1.4, -25; 128 to 1,024 (533 MB) -24.
+SAVED_BYTES = 32 << 20
+SAVED_BYTES_EACH = 5 << 20      # and these for each sequence, of SAVED_SEQUENCES at most
+SAVED_SEQUENCES = 40
+# Tokens a sequence from which a step is worth more as a prompt: its own columns fill the products by then. 24 sequences of 8, 40 and 200 new tokens behind
+# 2,000 shared ones: 28, 46, 157 us shared, 34, 38, 121 us separate; behind 1,000: 23, 40, 128 and 23, 27, 80 us.
 MANY_TOKENS = 8
 
 
@@ -173,11 +185,11 @@ def pays(meta, kv, nq, nkv, hd, dtype):
 def _ends_sooner(meta, nkv, hd, dtype):
     if meta.shared is None:
         return False
-    if dtype == torch.float32:
+    if dtype == torch.float32:          # (8 sequences of 128 tokens: 11 us shared, 17 separate; of 2,048: 17 and 103)
         return True
     if meta.max_new > 1 and meta.num_tokens > MANY_TOKENS * meta.num_seqs:
         return False
-    return _saved(meta, nkv, hd, dtype) >= SAVED_BYTES
+    return _saved(meta, nkv, hd, dtype) >= SAVED_BYTES + SAVED_BYTES_EACH * min(meta.num_seqs, SAVED_SEQUENCES)
 
 
 def _plan_of(meta, nq, nkv, hd, dtype):

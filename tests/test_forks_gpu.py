@@ -23,6 +23,7 @@ def used(monkeypatch):
     """Shared pages are read together whatever they save (tiny models save little); counts the calls that do."""
     calls = []
     monkeypatch.setattr(shared, "SAVED_BYTES", 1)
+    monkeypatch.setattr(shared, "SAVED_BYTES_EACH", 0)
     monkeypatch.setattr(shared, "MANY_TOKENS", 1000)
     real = shared.attention
 
