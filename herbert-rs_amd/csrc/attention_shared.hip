@@ -680,7 +680,7 @@ attn_shared_join_kernel(const float* __restrict__ partial_o, const float* __rest
 #pragma unroll
             for (int u = 0; u < AHEAD; ++u) {
                 const float ws = __shfl(w, (s + u) % LANES, LANES);
-                const bool counts = s + u < here && ws != 0.f;
+                const bool counts = s + u < here;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) acc[e] = counts ? fmaf(ws, v[u][e], acc[e]) : acc[e];
             }

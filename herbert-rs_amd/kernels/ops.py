@@ -49,7 +49,7 @@ class stream_scope:
 
 def _stream():
     s = getattr(_scoped, "stream", None)
-    return s if s is not None else torch.cuda.current_stream().cuda_stream
+    return s if s is not None else torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())     # (no Stream object for a number: 2 us less a launch)
 
 
 _fits = None
@@ -71,6 +71,13 @@ def _check(t, name, dtype=None, shape=None):
         raise BackendError(f"{name} must be {dtype}, got {t.dtype}")
     if shape is not None and (len(shape) != t.dim() or any(s is not None and s != d for s, d in zip(shape, t.shape))):
         raise BackendError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
+
+
+def _check_device(what, *devices):
+    """Launches go to the current device: tensors of another one (`get_device()` of each) are refused."""
+    at = torch._C._cuda_getDevice()
+    if devices.count(at) != len(devices):
+        raise BackendError(f"{what}: tensors lie on GPUs {sorted(set(devices))}, the current one is {at}")
 
 
 def _ptr(t):
@@ -440,7 +447,7 @@ def token_logprobs(logits, tokens, chosen, entropy, ids=None, best=None, scratch
     entries and their log p, larger first, the lower id first among equals. logits f32 [R, V], tokens int32 [R] (one outside the
     vocabulary: NaN), chosen, entropy f32 [R], ids int32 and best f32 [R, n] with n <= 64 (both or neither). A
     row that holds NaN or +inf, or nothing above -inf, is no distribution: NaN, and the ids are -1.
-    `scratch` as `logprob_scratch` makes it (for at least R such rows), else it is allocated here."""
+    `scratch` as `logprob_scratch` makes it (for at least R such rows), for one call (or recorded graph) at a time; else memory of this call's own."""
     _check(logits, "logits", torch.float32, (None, None))
     R, V = logits.shape
     _check(tokens, "tokens", torch.int32, (R,))
@@ -455,6 +462,7 @@ def token_logprobs(logits, tokens, chosen, entropy, ids=None, best=None, scratch
         _check(best, "best", torch.float32, (R, top))
         if not 0 < top <= min(LOGPROB_MOST, V):
             raise BackendError(f"token_logprobs: 1 to {min(LOGPROB_MOST, V)} alternatives of {V} logits, not {top}")
+    _check_device("token_logprobs", logits.get_device(), tokens.get_device(), chosen.get_device(), entropy.get_device())
     chunks = -(-V // LOGPROB_CHUNK)
     stats = keys = None
     if chunks > 1:

@@ -35,8 +35,9 @@ SAVED_BYTES = 32 << 20
 SAVED_BYTES_EACH = 5 << 20      # and these for each sequence, of SAVED_SEQUENCES at most
 SAVED_SEQUENCES = 40
 # Tokens a sequence from which a step is worth more as a prompt: its own columns fill the products by then. 24 sequences of 8, 40 and 200 new tokens behind
-# 2,000 shared ones: 28, 46, 157 us shared, 34, 38, 121 us separate; behind 1,000: 23, 40, 128 and 23, 27, 80 us.
-MANY_TOKENS = 8
+# 2,000 shared ones: 28, 46, 157 us shared, 34, 38, 121 us separate; behind 1,000: 23, 40, 128 and 23, 27, 80 us. In float32 16 sequences of 8, 40 and
+# 200 behind 256: 15, 38, 135 us shared, 21, 33, 129 us separate; behind 2,000: 37, 128, 526 and 98, 146, 566 us.
+MANY_TOKENS = {torch.bfloat16: 8, torch.float32: 200}
 
 
 def supported(kv, nq, nkv, hd, dtype):
@@ -65,6 +66,8 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
     that a tile of more than 64 columns sees in part are items of their own."""
     starts, context = np.asarray(starts, dtype=np.int64), np.asarray(context, dtype=np.int64)
     counts = np.diff(starts)
+    if len(sharing.order) != len(counts):
+        raise BackendError(f"shared attention: pages shared by {len(sharing.order)} sequences in a step of {len(counts)}")
     row_of = np.concatenate([[0], np.cumsum(counts[sharing.order])])            # a sequence's first row in the order
     order = np.concatenate([np.arange(starts[i], starts[i + 1]) for i in sharing.order])
     tall = max(1, columns // group)
@@ -121,14 +124,14 @@ def _planned(meta, group, nkv, dtype, grid=1):
 
 
 class Plan:
-    """A plan on the GPU."""
+    """A plan on the GPU: of meta.shared as it is now."""
 
     def __init__(self, meta, group, nkv, dtype):
         items, order, part_start, parts, self.max_rows = _planned(meta, group, nkv, dtype)
         both = send(np.concatenate([a.ravel() for a in (items, order, part_start, parts)]), meta.positions.device)
         at = np.cumsum([a.size for a in (items, order, part_start, parts)])
         self.items, self.order, self.part_start, self.parts = both[:at[0]], both[at[0]:at[1]], both[at[1]:at[2]], both[at[2]:]
-        self.n_items, self.n_parts = len(items), len(parts)
+        self.sharing, self.n_items, self.n_parts = meta.shared, len(items), len(parts)
 
 
 class StaticPlan:
@@ -185,10 +188,10 @@ def pays(meta, kv, nq, nkv, hd, dtype):
 def _ends_sooner(meta, nkv, hd, dtype):
     if meta.shared is None:
         return False
+    if meta.max_new > 1 and meta.num_tokens > MANY_TOKENS[dtype] * meta.num_seqs:
+        return False
     if dtype == torch.float32:          # (8 sequences of 128 tokens: 11 us shared, 17 separate; of 2,048: 17 and 103)
         return True
-    if meta.max_new > 1 and meta.num_tokens > MANY_TOKENS * meta.num_seqs:
-        return False
     return _saved(meta, nkv, hd, dtype) >= SAVED_BYTES + SAVED_BYTES_EACH * min(meta.num_seqs, SAVED_SEQUENCES)
 
 
@@ -201,7 +204,8 @@ def _plan_of(meta, nq, nkv, hd, dtype):
             raise BackendError("shared attention: it does not pay for this step (see pays)")
         return found
     found = meta.derived.get(key)          # every layer's attention asks: worked out once a step
-    if found is None:
+    if found is None or found.sharing is not meta.shared:
+        mfma._not_while_recording("the plan of a step's shared pages")
         found = meta.derived[key] = Plan(meta, nq // nkv, nkv, dtype)
     return found
 
@@ -210,27 +214,36 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     """Causal attention of the step's tokens over their slots' pages, a page that several sequences share read once for all of
     them. q, out [T, nq hd] in the cache's dtype, bfloat16 (heads of 32, 64 or 128) or float32 (up to 256, a multiple of 4); meta.shared: a cache.SharedPages of
     the step's sequences. sinks f32 [nq]: the softmax's denominator of head h also holds exp(sinks[h]). softcap: a scaled score s
-    becomes softcap tanh(s / softcap)."""
+    becomes softcap tanh(s / softcap). scratch: a mfma.Scratch whose memory the partial results take, for one call (or recorded graph) at a
+    time; None: memory of this call's own. meta is used on the stream that it was packed on."""
     T = q.shape[0]
     if meta.shared is None:
         raise BackendError("shared attention: the sequences of this step share no pages")
     if not supported(kv, nq, nkv, hd, q.dtype):
         raise BackendError(f"shared attention refuses {nq}/{nkv} heads of {hd} in {q.dtype} over this cache")
-    _check(q, "q", kv.k.dtype, (T, nq * hd))
-    _check(out, "out", kv.k.dtype, (T, nq * hd))
-    pages = kv.k.shape[0]
-    _check(kv.k, "key pages", None, (pages, nkv, 64, hd))
-    _check(kv.v, "value pages", kv.k.dtype, (pages, nkv, hd, 64))
-    _check(kv.page_table, "page_table", torch.int32, (None, None))
+    keys, values, table = kv.k, kv.v, kv.page_table
+    _check(q, "q", keys.dtype, (T, nq * hd))
+    _check(out, "out", keys.dtype, (T, nq * hd))
+    pages = keys.shape[0]
+    _check(keys, "key pages", None, (pages, nkv, 64, hd))
+    _check(values, "value pages", keys.dtype, (pages, nkv, hd, 64))
+    _check(table, "page_table", torch.int32, (None, None))
     _check(meta.positions, "positions", torch.int32, (T,))
     _check(meta.seq_of, "seq_of", torch.int32, (T,))
     _check(meta.slots, "slots", torch.int32, (meta.num_seqs,))
     if sinks is not None:
         _check(sinks, "sinks", torch.float32, (nq,))
+    ops._check_device("shared attention", q.get_device(), out.get_device(), keys.get_device(), values.get_device(), table.get_device(),
+                      meta.positions.get_device())
+    if meta.max_context > 64 * table.shape[1]:
+        raise BackendError(f"shared attention: a context of {meta.max_context} tokens does not fit a table of {table.shape[1]} pages")
     p = _plan_of(meta, nq, nkv, hd, q.dtype)
-    po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
-    lib.call("attention_shared", "hb_attn_shared", q.data_ptr(), kv.k.data_ptr(), kv.v.data_ptr(), out.data_ptr(), ops.dtype_code(q),
+    if scratch is None:
+        po, pml = (torch.empty(p.n_parts * nq * n, dtype=torch.float32, device=q.device) for n in (hd, 2))
+    else:
+        po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
+    lib.call("attention_shared", "hb_attn_shared", q.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr(), ops.dtype_code(q),
              po.data_ptr(), pml.data_ptr(), p.items.data_ptr(), p.n_items, p.max_rows, 1 if meta.max_new > 1 else 0, p.order.data_ptr(), p.part_start.data_ptr(),
-             p.parts.data_ptr(), T, meta.positions.data_ptr(), meta.seq_of.data_ptr(), meta.slots.data_ptr(), kv.page_table.data_ptr(),
-             kv.page_table.shape[1], nq, nkv, hd, float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
+             p.parts.data_ptr(), T, meta.positions.data_ptr(), meta.seq_of.data_ptr(), meta.slots.data_ptr(), table.data_ptr(),
+             table.shape[1], nq, nkv, hd, float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
              _stream())

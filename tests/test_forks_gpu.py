@@ -24,7 +24,7 @@ def used(monkeypatch):
     calls = []
     monkeypatch.setattr(shared, "SAVED_BYTES", 1)
     monkeypatch.setattr(shared, "SAVED_BYTES_EACH", 0)
-    monkeypatch.setattr(shared, "MANY_TOKENS", 1000)
+    monkeypatch.setattr(shared, "MANY_TOKENS", {torch.bfloat16: 1000, torch.float32: 1000})
     real = shared.attention
 
     def counted(*args, **kw):

@@ -167,6 +167,13 @@ def test_scratch_that_is_too_small_and_shapes_that_do_not_fit():
         ops.token_logprobs(logits, tokens, torch.empty(4, device="cuda"), torch.empty(4, device="cuda"), ids=torch.empty(4, 2, dtype=torch.int32, device="cuda"))
 
 
+def test_tensors_of_another_gpu_than_the_current_one_are_refused(monkeypatch):
+    logits, tokens = random_logits(2, 300, 6)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 3)
+    with pytest.raises(BackendError, match="tensors lie on GPUs .0., the current one is 3"):
+        ops.token_logprobs(logits, tokens, torch.empty(2, device="cuda:0"), torch.empty(2, device="cuda:0"))
+
+
 def test_a_captured_call_replays_alike():
     logits, tokens = random_logits(7, 30000, 7)
     scratch = ops.logprob_scratch(7, 30000, 5, logits.device)

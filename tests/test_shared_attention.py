@@ -146,6 +146,8 @@ def test_what_the_shared_attention_refuses():
     for other in (windowed, keys_only, LayerKV(kv.k.bfloat16(), kv.v.bfloat16(), kv.page_table, 64, 0)):
         with pytest.raises(BackendError, match="refuses"):
             shared.attention(q, meta, other, q, 4, 2, 64, 0.125)
+    with pytest.raises(BackendError, match="shared by 2 sequences in a step of 3"):
+        shared.plan([0, 1, 2, 3], [65, 65, 65], [0, 1, 2], meta.shared, 2, 2, 128, 512)
 
 
 def call(**changed):

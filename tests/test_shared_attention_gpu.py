@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from herbert_rs_amd.cache import LayerKV
+from herbert_rs_amd.errors import BackendError, NeedsEagerStep
 from herbert_rs_amd.kernels import mfma, shared
 
 from .conftest import observe
@@ -189,3 +191,78 @@ def test_a_captured_call_replays_alike():
             torch.cuda.synchronize()
         graph.replay()
         assert torch.equal(again, out)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_a_value_without_a_size_is_not_lost_behind_a_weight_of_nothing(dtype):
+    """One key holds all the weight (its score is hundreds above the others): 0 x inf in another page is NaN, as in the formula's own arithmetic."""
+    q, meta, kv, out, table = run(plain_samples(4, 5), [5 * 64 + 9] * 4, [1] * 4, 2, 1, 64, dtype)
+    q.fill_(4.0)
+    kv.k[:] = 0.0
+    kv.k[table[:, 5], 0, 3] = 40.0                       # score 1,280
+    kv.v[table[0, 0], 0, 7, 11] = float("inf")
+    shared.attention(q, meta, kv, out, 2, 1, 64, 0.125)
+    bad = ~torch.isfinite(out.view(4, 2, 64))
+    assert bad[:, :, 7].all() and bad.sum() == 8
+
+
+def test_a_call_without_scratch_is_its_own_on_every_stream():
+    """Two streams at a time, no scratch given: their partial results do not meet."""
+    case = (plain_samples(20, 9), [64 * 9 + i for i in range(20)], [1] * 20, 8, 2, 128, BF)
+    made = [run(*case), run(plain_samples(20, 5), [64 * 5 + 3 * i for i in range(20)], [1] * 20, 8, 2, 128, BF)]
+    want = [m[3].clone() for m in made]
+    outs = [[torch.empty_like(m[3]) for _ in range(12)] for m in made]
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(12):
+        for (q, meta, kv, _, _), side, out in zip(made, sides, outs):
+            with torch.cuda.stream(side):
+                shared.attention(q, meta, kv, out[i], 8, 2, 128, 128 ** -0.5)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, w) for out, w in zip(outs, want) for o in out)
+
+
+def test_a_plan_follows_what_is_shared_and_is_not_made_while_recording():
+    seqs, held = plain_samples(6, 4), [64 * 4 + i for i in range(6)]
+    q, meta, kv, out, table = run(seqs, held, [1] * 6, 4, 2, 64, BF)
+    from herbert_rs_amd.cache import SharedPages
+    nodes = meta.shared.nodes
+    assert nodes[0][1] == 6
+    # the same step with the first three pages shared alone: other sums, the same result within the rounding of the outputs
+    first = [(0, 6, 0, 3)] + [(i, 1, 3, -1) for i in range(6)]
+    meta.shared = SharedPages(meta.shared.order, first)
+    again = torch.empty_like(out)
+    shared.attention(q, meta, kv, again, 4, 2, 64, 0.125)
+    assert len([v for k, v in meta.derived.items() if k[0] == "shared_plan"]) == 1
+    assert next(v for k, v in meta.derived.items() if k[0] == "shared_plan").sharing is meta.shared
+    compare(again, reference(q, kv, table, held, [1] * 6, 4, 2, 64, 0.125), BF, 64, max(held) + 1, "another cut")
+    fresh = step(table, held, [1] * 6, dev())
+    scratch = mfma.Scratch()
+    shared.attention(q, meta, kv, again, 4, 2, 64, 0.125, scratch=scratch)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        graph.capture_begin()
+        try:
+            with pytest.raises(NeedsEagerStep, match="plan"):
+                shared.attention(q, fresh, kv, again, 4, 2, 64, 0.125, scratch=scratch)
+            again.zero_()
+        finally:
+            graph.capture_end()
+    torch.cuda.synchronize()
+
+
+def test_calls_refused_before_a_launch(monkeypatch):
+    q, meta, kv, out, table = run(plain_samples(3, 2), [128 + 9, 128, 128 + 40], [1] * 3, 4, 2, 64, BF)
+    with pytest.raises(BackendError, match="does not fit a table of 2"):
+        shared.attention(q, meta, LayerKV(kv.k, kv.v, kv.page_table[:, :2].contiguous(), 64, 0), out, 4, 2, 64, 0.125)
+    with pytest.raises(BackendError, match="contiguous"):
+        shared.attention(q, meta, LayerKV(kv.k.transpose(2, 3), kv.v, kv.page_table, 64, 0), out, 4, 2, 64, 0.125)
+    with pytest.raises(BackendError, match="out must be"):
+        shared.attention(q, meta, kv, out.float(), 4, 2, 64, 0.125)
+    with pytest.raises(BackendError, match="sinks must"):
+        shared.attention(q, meta, kv, out, 4, 2, 64, 0.125, sinks=torch.zeros(3, device="cuda"))
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 5)
+    with pytest.raises(BackendError, match="tensors lie on GPUs .0., the current one is 5"):
+        shared.attention(q, meta, kv, out, 4, 2, 64, 0.125)
