@@ -19,7 +19,8 @@ HB_MODULE_ERROR_SLOT()
 #define THREADS 256
 #define PER (CHUNK / THREADS)
 #define MAX_TOP 64
-#define LISTED 1024        // candidates that are ranked at once
+#define LISTED 1024        // candidates that are listed
+#define RANKED 128         // and ranked
 
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
 
@@ -51,17 +52,43 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int off) {
 }
 
 struct Selecting {
-    uint64_t list[LISTED];
-    uint64_t groups[64], wave_best[THREADS / 64];
+    uint64_t list[LISTED], last[RANKED];
+    uint64_t groups[64];
     int above[THREADS / 64][64], count;
 };
 
+// A bound from which there are `most` keys or fewer, but `top` at least: between lo, from which there are `count`, and hi, from which there
+// are fewer than `top`, by halving. of(bound): how many of the thread's keys lie at or above a bound.
+template <class Of>
+__device__ uint64_t narrowed(Selecting& sh, int top, int most, uint64_t lo, uint64_t hi, int count, Of of) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    while (count > most && hi - lo > 1) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        int n = of(mid);
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
+        if (lane == 0) sh.above[wave][0] = n;
+        __syncthreads();
+        n = (sh.above[0][0] + sh.above[1][0]) + (sh.above[2][0] + sh.above[3][0]);
+        __syncthreads();
+        if (n >= top) {
+            lo = mid;
+            count = n;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
 // The `top` largest of the keys that a workgroup holds, written by put(rank, key): ranks 0 .. top - 1, those that there is no key
-// for with the key 0. largest: the thread's own largest key; each(bound, f) hands f the thread's keys from bound on, and may hand it others.
-// The n-th largest of the 64 largest keys of four threads each bounds the n largest of all from below, and few keys lie at or above it: those
-// are listed and ranked by counting. Where more are than the list holds, the largest is looked for `top` times.
-template <class Each, class Put>
-__device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, Put put) {
+// for with the key 0. largest: the thread's own largest key; each(bound, f) hands f the thread's keys from bound on, and may hand it others;
+// counted(bound): how many they are.
+// The n-th largest of the 64 largest keys of four threads each bounds the n largest of all from below. The keys at or above it are listed,
+// mostly few; where they are many, the bound is moved up by halving first (an order of the keys in memory that puts the largest side by side
+// leaves up to 16 for each of them). The last ones are ranked by counting.
+template <class Each, class Counted, class Put>
+__device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, Counted counted, Put put) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     uint64_t g = largest;
 #pragma unroll
@@ -81,43 +108,58 @@ __device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, 
     above = (sh.above[0][lane] + sh.above[1][lane]) + (sh.above[2][lane] + sh.above[3][lane]);
     // (keys are of different ids, only 0 may be there twice: no group has the n-th place, and every key counts)
     const uint64_t found = __builtin_amdgcn_ballot_w64(above == top - 1 && of_lane != 0);
-    const uint64_t bound = found ? sh.groups[__ffsll((unsigned long long)found) - 1] : 1;
-    each(bound, [&](uint64_t key) {
-        if (key >= bound) {
-            const int at = atomicAdd(&sh.count, 1);
-            if (at < LISTED) sh.list[at] = key;
-        }
-    });
-    __syncthreads();
-    const int count = sh.count;
-    if (count <= LISTED) {
-        for (int i = tid; i < count; i += THREADS) {
-            const uint64_t mine = sh.list[i];
-            int above = 0;
-#pragma unroll 8
-            for (int j = 0; j < count; ++j) above += sh.list[j] > mine ? 1 : 0;
-            if (above < top) put(above, mine);
-        }
-        for (int i = count + tid; i < top; i += THREADS) put(i, (uint64_t)0);
-        return;
-    }
-    uint64_t before = ~(uint64_t)0;
-    for (int n = 0; n < top; ++n) {
-        uint64_t best = 0;
-        each(1, [&](uint64_t key) { best = key < before && key > best ? key : best; });
+    uint64_t bound = found ? sh.groups[__ffsll((unsigned long long)found) - 1] : 1;
+    auto list = [&](uint64_t* to, int room, auto keys) {
+        keys([&](uint64_t key) {
+            if (key >= bound) {
+                const int at = atomicAdd(&sh.count, 1);
+                if (at < room) to[at] = key;
+            }
+        });
+        __syncthreads();
+        return sh.count;
+    };
+    auto of_thread = [&](auto f) { each(bound, f); };
+    int count = list(sh.list, LISTED, of_thread);
+    const uint64_t* ranked = sh.list;
+    if (count > RANKED) {
+        uint64_t hi = of_lane;
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) {
-            const uint64_t o = shfl_xor_u64(best, off);
-            best = o > best ? o : best;
+            const uint64_t o = shfl_xor_u64(hi, off);
+            hi = o > hi ? o : hi;
         }
-        if (lane == 0) sh.wave_best[wave] = best;
+        ++hi;
+        const bool listed = count <= LISTED;
+        const int n = count;
+        auto of_list = [&](auto f) {
+            for (int i = tid; i < n; i += THREADS) f(sh.list[i]);
+        };
+        if (listed)
+            bound = narrowed(sh, top, RANKED, bound, hi, n, [&](uint64_t from) {
+                int c = 0;
+                of_list([&](uint64_t key) { c += key >= from ? 1 : 0; });
+                return c;
+            });
+        else
+            bound = narrowed(sh, top, RANKED, bound, hi, n, counted);
+        __syncthreads();                                  // (the count has been read)
+        if (tid == 0) sh.count = 0;
         __syncthreads();
-        best = sh.wave_best[0];
-        for (int w = 1; w < THREADS / 64; ++w) best = sh.wave_best[w] > best ? sh.wave_best[w] : best;
-        __syncthreads();
-        if (tid == 0) put(n, best);
-        before = best;
+        count = listed ? list(sh.last, RANKED, of_list) : list(sh.last, RANKED, of_thread);
+        if (count > RANKED) count = RANKED;
+        ranked = sh.last;
     }
+    int each_by = 1;                                      // threads that count for one of them
+    while (each_by < 64 && 2 * each_by * count <= THREADS) each_by *= 2;
+    const int i = tid / each_by, part = tid % each_by;    // (THREADS / each_by >= count)
+    const uint64_t mine = ranked[i < count ? i : 0];
+    above = 0;
+#pragma unroll 8
+    for (int j = part; j < count; j += each_by) above += ranked[j] > mine ? 1 : 0;
+    for (int off = each_by / 2; off > 0; off >>= 1) above += __shfl_xor(above, off, 64);
+    if (i < count && part == 0 && above < top) put(above, mine);
+    for (int n = count + tid; n < top; n += THREADS) put(n, (uint64_t)0);
 }
 
 // A row's results from its m, S and T: what the row's threads share.
@@ -143,9 +185,9 @@ __device__ __forceinline__ void leave_top(const Row& r, uint64_t key, int* id, f
     *best = r.bad ? __uint_as_float(0x7fc00000u) : (value_of(key) - r.m) - r.log_s;
 }
 
-// stats [row][chunk]: (m, S, T); keys [row][chunk][top]. One chunk a row: the row's results themselves.
+// stats [row][chunk]: (m, S, T); keys [row][rank][chunk], so that neighbours are alike in rank. One chunk a row: the row's results themselves.
 template <bool TOP>
-__global__ void __launch_bounds__(THREADS)
+__global__ void __launch_bounds__(THREADS, 8)
 logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restrict__ tokens, float* __restrict__ chosen,
                      float* __restrict__ entropy, int* __restrict__ ids, float* __restrict__ best, int top, int chunks,
                      float4* __restrict__ stats, uint64_t* __restrict__ keys) {
@@ -211,8 +253,18 @@ logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restr
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 if (x[i] >= least) f(id_at(i) < len ? key_of(x[i], first + id_at(i)) : (uint64_t)0);
+        }, [&](uint64_t bound) {
+            // (a bound need not be a logit's key: below all of them, and between those of -0, of which there are none, and 0)
+            const uint64_t lowest = (uint64_t)0x007fffffu << 32, zero = (uint64_t)0x80000000u << 32;
+            bound = bound < lowest ? lowest : (uint32_t)(bound >> 32) == 0x7fffffffu ? zero : bound;
+            const float least = value_of(bound);
+            const int last = (int)min(~(uint32_t)bound, (uint32_t)(first + len - 1)) - first;
+            int n = 0;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) n += (x[i] > least || (x[i] == least && id_at(i) <= last)) ? 1 : 0;
+            return n;
         }, [&](int rank, uint64_t key) {
-            if (chunks > 1) keys[(r * chunks + chunk) * top + rank] = key;
+            if (chunks > 1) keys[(r * top + rank) * chunks + chunk] = key;
             else leave_top(whole, key, ids + r * top + rank, best + r * top + rank);
         });
     }
@@ -261,6 +313,10 @@ logprob_row_kernel(const float* __restrict__ logits, int V, const int* __restric
         for (int i = tid; i < n; i += THREADS) largest = keys[i] > largest ? keys[i] : largest;
         select_top(sh, top, largest, [&](uint64_t, auto f) {
             for (int i = tid; i < n; i += THREADS) f(keys[i]);
+        }, [&](uint64_t bound) {
+            int c = 0;
+            for (int i = tid; i < n; i += THREADS) c += keys[i] >= bound ? 1 : 0;
+            return c;
         }, [&](int rank, uint64_t key) { leave_top(whole, key, ids + r * top + rank, best + r * top + rank); });
     }
 }

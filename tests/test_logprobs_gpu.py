@@ -93,6 +93,23 @@ def test_sorted_rows(V):
         check(logits, torch.tensor([V - 1, 0, 5], dtype=torch.int32, device="cuda"), top)
 
 
+@pytest.mark.parametrize("V, top", [(1121, 64), (4096, 33), (4096, 64), (40000, 64), (151936, 64)])
+def test_more_candidates_than_are_ranked(V, top):
+    """Rows in which one bound from the largest of a few threads' logits leaves hundreds of candidates, or more than are listed: many equal
+    ones, zeros of both signs, a few finite ones among banned ones, neighbours that differ in the last bit, and all of it below zero."""
+    logits, tokens = random_logits(8, V, V + top)
+    at = torch.arange(V, device="cuda")
+    logits[1] = torch.where(at % 7 < 6, 1.0, logits[1])
+    logits[2] = torch.where(at % 3 == 0, -0.0, torch.where(at % 3 == 1, 0.0, -logits[2].abs() - 1))
+    logits[3] = torch.where((at // 4) % 256 < 4, logits[3], -float("inf"))
+    logits[3, 0] = 0.0
+    logits[4] = (torch.full((V,), 1.0, device="cuda").view(torch.int32) + (at * 48271 % 8191).int()).view(torch.float32)
+    logits[5] = -(torch.full((V,), 3.0, device="cuda").view(torch.int32) + (at * 48271 % 8191).int()).view(torch.float32)
+    logits[6] = torch.where((at // 4) % 256 < 200, 5.0 + logits[6].abs(), -90.0)
+    logits[7] = torch.where(at < top // 2, 0.0, -float("inf"))
+    check(logits, tokens, top)
+
+
 def test_the_largest_logits_all_with_the_same_threads():
     """A thread of the first kernel holds 16 logits of a chunk: four threads that hold the 64 largest of their chunk, and a row in which
     a few threads hold so many that the list of candidates does not hold them."""
