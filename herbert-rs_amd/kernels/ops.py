@@ -428,7 +428,7 @@ def force_tokens(logits, rows, tokens):
              len(rows), _stream())
 
 
-LOGPROB_CHUNK = 4096
+LOGPROB_CHUNK = 4096         # logits of a workgroup (csrc/logprobs.hip)
 LOGPROB_MOST = 64            # alternatives a row
 
 
