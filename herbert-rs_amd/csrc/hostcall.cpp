@@ -53,7 +53,7 @@ PyObject* make_entry(PyObject*, PyObject* args) {
     return PyCapsule_New(new Entry(e), ENTRY, free_entry);
 }
 
-// invoke(entry, arguments...): what the function returns. None is a null pointer; the interpreter is free meanwhile.
+// invoke(entry, arguments...): what the function returns. None is a null pointer, a tensor its memory; the interpreter is free meanwhile.
 PyObject* invoke(PyObject*, PyObject* const* args, Py_ssize_t n) {
     Entry* e = n > 0 ? (Entry*)PyCapsule_GetPointer(args[0], ENTRY) : nullptr;
     if (!e) {
@@ -68,8 +68,16 @@ PyObject* invoke(PyObject*, PyObject* const* args, Py_ssize_t n) {
         PyObject* a = args[1 + i];
         if (e->is_float[i]) {
             f[nf++] = (float)PyFloat_AsDouble(a);
+        } else if (a == Py_None) {
+            w[nw++] = 0;
+        } else if (!PyLong_Check(a) && THPVariable_Check(a)) {
+            try {
+                w[nw++] = (uint64_t)THPVariable_Unpack(a).data_ptr();
+            } catch (const std::exception& ex) {
+                return PyErr_Format(PyExc_TypeError, "argument %d has no memory: %s", i, ex.what());
+            }
         } else {
-            w[nw++] = a == Py_None ? 0 : PyLong_AsUnsignedLongLongMask(a);
+            w[nw++] = PyLong_AsUnsignedLongLongMask(a);
         }
     }
     if (PyErr_Occurred()) return nullptr;
@@ -113,9 +121,34 @@ PyObject* fits(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return PyBool_FromLong(is);
 }
 
+// all_fit(tensor, dtype, shape, tensor, dtype, shape, ...): the GPU that all of them lie on if each fits, else -1, and the caller says
+// what is wrong.
+PyObject* all_fit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    if (n % 3 != 0) {
+        PyErr_SetString(PyExc_TypeError, "tensors, each with a type and a shape, are needed");
+        return nullptr;
+    }
+    long at = -1;
+    bool is = true;
+    try {
+        for (Py_ssize_t i = 0; is && i < n; i += 3) {
+            is = THPVariable_Check(args[i]) && has_form(THPVariable_Unpack(args[i]), args[i + 1], args[i + 2]);
+            if (!is) break;
+            const long device = THPVariable_Unpack(args[i]).get_device();
+            is = at < 0 || at == device;
+            at = device;
+        }
+    } catch (const std::exception&) {
+        is = false;
+    }
+    PyErr_Clear();
+    return PyLong_FromLong(is ? at : -1);
+}
+
 PyMethodDef methods[] = {{"entry", make_entry, METH_VARARGS, nullptr},
                          {"invoke", (PyCFunction)(void*)invoke, METH_FASTCALL, nullptr},
                          {"fits", (PyCFunction)(void*)fits, METH_FASTCALL, nullptr},
+                         {"all_fit", (PyCFunction)(void*)all_fit, METH_FASTCALL, nullptr},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "hostcall", nullptr, -1, methods};
 

@@ -73,11 +73,21 @@ def _check(t, name, dtype=None, shape=None):
         raise BackendError(f"{name} must have shape {list(shape)}, got {list(t.shape)}")
 
 
-def _check_device(what, *devices):
-    """Launches go to the current device: tensors of another one (`get_device()` of each) are refused."""
-    at = torch._C._cuda_getDevice()
-    if devices.count(at) != len(devices):
-        raise BackendError(f"{what}: tensors lie on GPUs {sorted(set(devices))}, the current one is {at}")
+_all_fit = None
+
+
+def _check_all(what, names, *operands):
+    """`_check` of several operands (tensor, dtype, shape, one after another) at once, which all have to lie on the current device: that is where
+    the launch goes."""
+    global _all_fit
+    if _all_fit is None:
+        _all_fit = lib.host().all_fit
+    at = _all_fit(*operands)
+    if at >= 0 and at == torch._C._cuda_getDevice():
+        return
+    for name, t, dtype, shape in zip(names, operands[::3], operands[1::3], operands[2::3]):
+        _check(t, name, dtype, shape)
+    raise BackendError(f"{what}: tensors lie on GPUs {sorted({t.get_device() for t in operands[::3]})}, the current one is {torch._C._cuda_getDevice()}")
 
 
 def _ptr(t):
@@ -448,21 +458,17 @@ def token_logprobs(logits, tokens, chosen, entropy, ids=None, best=None, scratch
     vocabulary: NaN), chosen, entropy f32 [R], ids int32 and best f32 [R, n] with n <= 64 (both or neither). A
     row that holds NaN or +inf, or nothing above -inf, is no distribution: NaN, and the ids are -1.
     `scratch` as `logprob_scratch` makes it (for at least R such rows), for one call (or recorded graph) at a time; else memory of this call's own."""
-    _check(logits, "logits", torch.float32, (None, None))
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2:
+        _check(logits, "logits", torch.float32, (None, None))
     R, V = logits.shape
-    _check(tokens, "tokens", torch.int32, (R,))
-    _check(chosen, "chosen", torch.float32, (R,))
-    _check(entropy, "entropy", torch.float32, (R,))
     if (ids is None) != (best is None):
         raise BackendError("token_logprobs: alternatives come as ids and log probabilities together")
-    top = 0
-    if ids is not None:
-        _check(ids, "ids", torch.int32, (R, None))
-        top = ids.shape[1]
-        _check(best, "best", torch.float32, (R, top))
-        if not 0 < top <= min(LOGPROB_MOST, V):
-            raise BackendError(f"token_logprobs: 1 to {min(LOGPROB_MOST, V)} alternatives of {V} logits, not {top}")
-    _check_device("token_logprobs", logits.get_device(), tokens.get_device(), chosen.get_device(), entropy.get_device())
+    top = 0 if ids is None else ids.shape[-1] if ids.dim() else 0
+    alternatives = () if ids is None else (ids, torch.int32, (R, top), best, torch.float32, (R, top))
+    _check_all("token_logprobs", ("logits", "tokens", "chosen", "entropy", "ids", "best"), logits, torch.float32, (R, V), tokens, torch.int32, (R,),
+               chosen, torch.float32, (R,), entropy, torch.float32, (R,), *alternatives)
+    if ids is not None and not 0 < top <= min(LOGPROB_MOST, V):
+        raise BackendError(f"token_logprobs: 1 to {min(LOGPROB_MOST, V)} alternatives of {V} logits, not {top}")
     chunks = -(-V // LOGPROB_CHUNK)
     stats = keys = None
     if chunks > 1:
@@ -471,8 +477,7 @@ def token_logprobs(logits, tokens, chosen, entropy, ids=None, best=None, scratch
         _check(keys, "candidates", torch.int64, (None,))
         if stats.numel() < R * chunks * 4 or keys.numel() < R * chunks * top:
             raise BackendError("token_logprobs: the scratch is too small for these logits")
-    lib.call("logprobs", "hb_token_logprobs", logits.data_ptr(), R, V, tokens.data_ptr(), chosen.data_ptr(), entropy.data_ptr(),
-             _ptr(ids), _ptr(best), top, _ptr(stats), _ptr(keys), _stream())
+    lib.call("logprobs", "hb_token_logprobs", logits, R, V, tokens, chosen, entropy, ids, best, top, stats, keys, _stream())
 
 
 def layernorm(x, weight, out, eps, rows=None, delta=None, mult=1.0):

@@ -11,7 +11,7 @@ import torch
 from ..errors import BackendError
 from ..hosted import send, send_into
 from . import lib, mfma, ops
-from .ops import _check, _stream
+from .ops import _stream
 
 _P, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 lib.register_signatures("attention_shared", {
@@ -25,6 +25,7 @@ F32_MOST_DIM = 256
 # bfloat16: 128 answers to 32,768 tokens 110, 95 and 89 us, 64 to 8,192 37, 33 and 33 us, 12 continuations of a text of 2,000 tokens
 # 46, 44 and 46 us.
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
+OPERANDS = ("q", "out", "key pages", "value pages", "page_table", "positions", "seq_of", "slots", "sinks")
 MASKED_COLUMNS = 64             # of an item in whose pages are places that some of its rows see and others do not: the wide ones ask no mask
 # The attention of one sequence after another also normalizes, rotates and writes what the projection gave; before the shared one that is a kernel of its
 # own. Bytes that need not be read again from which the shared one ends sooner all the same, in a model's decode steps (36 layers of 32 heads of
@@ -222,19 +223,11 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     if not supported(kv, nq, nkv, hd, q.dtype):
         raise BackendError(f"shared attention refuses {nq}/{nkv} heads of {hd} in {q.dtype} over this cache")
     keys, values, table = kv.k, kv.v, kv.page_table
-    _check(q, "q", keys.dtype, (T, nq * hd))
-    _check(out, "out", keys.dtype, (T, nq * hd))
-    pages = keys.shape[0]
-    _check(keys, "key pages", None, (pages, nkv, 64, hd))
-    _check(values, "value pages", keys.dtype, (pages, nkv, hd, 64))
-    _check(table, "page_table", torch.int32, (None, None))
-    _check(meta.positions, "positions", torch.int32, (T,))
-    _check(meta.seq_of, "seq_of", torch.int32, (T,))
-    _check(meta.slots, "slots", torch.int32, (meta.num_seqs,))
-    if sinks is not None:
-        _check(sinks, "sinks", torch.float32, (nq,))
-    ops._check_device("shared attention", q.get_device(), out.get_device(), keys.get_device(), values.get_device(), table.get_device(),
-                      meta.positions.get_device())
+    pages, dtype, i32 = keys.shape[0], keys.dtype, torch.int32
+    further = () if sinks is None else (sinks, torch.float32, (nq,))
+    ops._check_all("shared attention", OPERANDS, q, dtype, (T, nq * hd), out, dtype, (T, nq * hd), keys, None, (pages, nkv, 64, hd),
+                   values, dtype, (pages, nkv, hd, 64), table, i32, (None, None), meta.positions, i32, (T,), meta.seq_of, i32, (T,),
+                   meta.slots, i32, (meta.num_seqs,), *further)
     if meta.max_context > 64 * table.shape[1]:
         raise BackendError(f"shared attention: a context of {meta.max_context} tokens does not fit a table of {table.shape[1]} pages")
     p = _plan_of(meta, nq, nkv, hd, q.dtype)
@@ -242,8 +235,6 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
         po, pml = (torch.empty(p.n_parts * nq * n, dtype=torch.float32, device=q.device) for n in (hd, 2))
     else:
         po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
-    lib.call("attention_shared", "hb_attn_shared", q.data_ptr(), keys.data_ptr(), values.data_ptr(), out.data_ptr(), ops.dtype_code(q),
-             po.data_ptr(), pml.data_ptr(), p.items.data_ptr(), p.n_items, p.max_rows, 1 if meta.max_new > 1 else 0, p.order.data_ptr(), p.part_start.data_ptr(),
-             p.parts.data_ptr(), T, meta.positions.data_ptr(), meta.seq_of.data_ptr(), meta.slots.data_ptr(), table.data_ptr(),
-             table.shape[1], nq, nkv, hd, float(scale), float(softcap or 0.0), None if sinks is None else sinks.data_ptr(),
-             _stream())
+    lib.call("attention_shared", "hb_attn_shared", q, keys, values, out, ops.dtype_code(q), po, pml, p.items, p.n_items, p.max_rows,
+             1 if meta.max_new > 1 else 0, p.order, p.part_start, p.parts, T, meta.positions, meta.seq_of, meta.slots, table, table.shape[1],
+             nq, nkv, hd, float(scale), float(softcap or 0.0), sinks, _stream())
