@@ -252,13 +252,17 @@ __global__ void qk_norm_rope_write_kernel(
 }
 
 // The same for many tokens (prompts), bfloat16 output, rotation over the whole head or none,
-// head size in steps of 8 up to 128, rows of the projection 16-byte aligned: a workgroup takes 64
+// head size in steps of 8 up to 128, rows of the projection 16-byte aligned: a workgroup takes 16
 // consecutive tokens of one head. Query and key heads: half a wave a token, 16 bytes a lane.
-// Value heads go through LDS, so that the transposed pages are written along the tokens: lane =
-// token, 64 consecutive tokens of a page are one 128-byte line.
+// Value heads go through LDS, so that the transposed pages are written along the tokens: 16 lanes
+// the 32 bytes of a page's row.
+// Bound by latency and by bytes. 48 heads of 128, one slice and four, against tiles of 64 tokens (a whole line of a page's row, but
+// few workgroups): 64 sequences of one token 5.2 and 5.2 us, 13.3 and 20.5; prompts of 512 6.9 and 11.9, 12.1 and 16.8; 2,048 19.1 and 34.2, 24.0 and
+// 39.3; 16,384 182 and 405, 194 and 413.
 // QS > 1: the projection was cut into QS slices of K whose sums lie slice_stride floats apart
 // behind qkv; they are added up in their order as they are loaded.
 #define HB_TILED_HEAD_DIM 128
+#define HB_TILED_TOKENS 16
 template <class TQ, class TC, int QS>
 __global__ void __launch_bounds__(256) qk_norm_rope_write_tiled_kernel(
     const float* __restrict__ qkv, int ld_qkv, size_t slice_stride, const float* __restrict__ q_norm_w,
@@ -267,8 +271,9 @@ __global__ void __launch_bounds__(256) qk_norm_rope_write_tiled_kernel(
     const int* __restrict__ page_table, int max_pages, int page_size, TQ* __restrict__ q_out,
     TC* __restrict__ k_cache, TC* __restrict__ v_cache, int T, int nq, int nkv, int hd, float eps,
     float q_temp_coef, int q_temp_every) {
-    __shared__ float vt[64][HB_TILED_HEAD_DIM + 1];
-    const int t0 = blockIdx.x * 64, h = blockIdx.y;
+    constexpr int TOK = HB_TILED_TOKENS, PASSES = TOK / 8;
+    __shared__ float vt[TOK][HB_TILED_HEAD_DIM + 1];
+    const int t0 = blockIdx.x * TOK, h = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const bool is_q = h < nq, is_v = h >= nq + nkv;
     const int half = hd / 2;
@@ -284,7 +289,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_write_tiled_kernel(
     if (is_v) {
         const int kvh = h - nq - nkv;
         const int q4 = hd / 4;                       // 16-byte chunks of a row
-        for (int idx = tid; idx < 64 * q4; idx += 256) {
+        for (int idx = tid; idx < TOK * q4; idx += 256) {
             const int r = idx / q4, c = (idx - r * q4) * 4;
             const int t = t0 + r;
             hb_f4 v = {0.f, 0.f, 0.f, 0.f};
@@ -293,18 +298,18 @@ __global__ void __launch_bounds__(256) qk_norm_rope_write_tiled_kernel(
             for (int e = 0; e < 4; ++e) vt[r][c + e] = v[e];
         }
         __syncthreads();
-        const int t = t0 + lane;
+        const int t = t0 + lane % TOK;
         if (t >= T) return;
         const int pos = positions[t];
         const int page = page_table[(size_t)slots[seq_of[t]] * max_pages + pos / page_size];
         TC* dst = v_cache + ((size_t)page * nkv + kvh) * page_size * hd + pos % page_size;
-        for (int d = wave; d < hd; d += 4) dst[(size_t)d * page_size] = hb_from_float<TC>(vt[lane][d]);
+        for (int d = tid / TOK; d < hd; d += 256 / TOK) dst[(size_t)d * page_size] = hb_from_float<TC>(vt[lane % TOK][d]);
         return;
     }
     // Query and key heads: half a wave a token, a lane four consecutive elements (16 bytes in, 8
     // out); the lanes l < hd / 8 hold the first half of the head, their partners l + hd / 8 the
-    // elements they are rotated with. A wave's 16 tokens go in two rounds of 8 (4 passes of 2
-    // tokens): all loads of a round go out before anything waits for them.
+    // elements they are rotated with. A wave's 4 tokens go in 2 passes: all loads go out before
+    // anything waits for them.
     const float* norm_w = is_q ? q_norm_w : k_norm_w;
     const int l = lane & 31, sub = lane >> 5;
     const int eighth = hd / 8;
@@ -315,63 +320,60 @@ __global__ void __launch_bounds__(256) qk_norm_rope_write_tiled_kernel(
     const int partner = (lane & 32) + (mine ? (first ? l + eighth : l - eighth) : l);
     hb_f4 w = {1.f, 1.f, 1.f, 1.f};
     if (norm_w && mine) w = *(const hb_f4*)(norm_w + d0);
+    hb_f4 x[PASSES], c[PASSES], sn[PASSES];
+    int pos[PASSES];
 #pragma unroll
-    for (int round = 0; round < 2; ++round) {
-        hb_f4 x[4], c[4], sn[4];
-        int pos[4];
+    for (int u = 0; u < PASSES; ++u) {
+        const int t = t0 + 2 * PASSES * wave + 2 * u + sub;
+        const int tc = t < T ? t : T - 1;
+        pos[u] = positions[tc];
+        x[u] = hb_f4{0.f, 0.f, 0.f, 0.f};
+        if (mine) x[u] = summed4(qkv + (size_t)tc * ld_qkv + (size_t)h * hd + d0);
+    }
+    if (cos_t) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int t = t0 + 16 * wave + 8 * round + 2 * u + sub;
-            const int tc = t < T ? t : T - 1;
-            pos[u] = positions[tc];
-            x[u] = hb_f4{0.f, 0.f, 0.f, 0.f};
-            if (mine) x[u] = summed4(qkv + (size_t)tc * ld_qkv + (size_t)h * hd + d0);
+        for (int u = 0; u < PASSES; ++u) {
+            c[u] = *(const hb_f4*)(cos_t + (size_t)pos[u] * half + j0);
+            sn[u] = *(const hb_f4*)(sin_t + (size_t)pos[u] * half + j0);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < PASSES; ++u) {
+        const int t = t0 + 2 * PASSES * wave + 2 * u + sub;
+        hb_f4 a = x[u];
+        if (norm_w) {
+            float ss = a[0] * a[0] + a[1] * a[1] + a[2] * a[2] + a[3] * a[3];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) ss += __shfl_xor(ss, d, 64);
+            const float inv = 1.0f / sqrtf(ss / (float)hd + eps);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) a[e] = a[e] * inv * w[e];
         }
         if (cos_t) {
+            hb_f4 o;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                c[u] = *(const hb_f4*)(cos_t + (size_t)pos[u] * half + j0);
-                sn[u] = *(const hb_f4*)(sin_t + (size_t)pos[u] * half + j0);
+            for (int e = 0; e < 4; ++e) {
+                const float other = __shfl(a[e], partner, 64);
+                // first half: x0 c - x1 s; second half: x0 s + x1 c (x0 the partner's element)
+                o[e] = first ? a[e] * c[u][e] - other * sn[u][e] : other * sn[u][e] + a[e] * c[u][e];
             }
+            a = o;
         }
+        if (!mine || t >= T) continue;
+        if (is_q && q_temp_every > 0) {
+            const float grow = hb_query_temperature(pos[u], q_temp_coef, q_temp_every);
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
-            const int t = t0 + 16 * wave + 8 * round + 2 * u + sub;
-            hb_f4 a = x[u];
-            if (norm_w) {
-                float ss = a[0] * a[0] + a[1] * a[1] + a[2] * a[2] + a[3] * a[3];
+            for (int e = 0; e < 4; ++e) a[e] *= grow;
+        }
+        TQ packed[4];
 #pragma unroll
-                for (int d = 1; d < 32; d <<= 1) ss += __shfl_xor(ss, d, 64);
-                const float inv = 1.0f / sqrtf(ss / (float)hd + eps);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = a[e] * inv * w[e];
-            }
-            if (cos_t) {
-                hb_f4 o;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float other = __shfl(a[e], partner, 64);
-                    // first half: x0 c - x1 s; second half: x0 s + x1 c (x0 the partner's element)
-                    o[e] = first ? a[e] * c[u][e] - other * sn[u][e] : other * sn[u][e] + a[e] * c[u][e];
-                }
-                a = o;
-            }
-            if (!mine || t >= T) continue;
-            if (is_q && q_temp_every > 0) {
-                const float grow = hb_query_temperature(pos[u], q_temp_coef, q_temp_every);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] *= grow;
-            }
-            TQ packed[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) packed[e] = hb_from_float<TQ>(a[e]);
-            if (is_q) {
-                *(uint2*)(q_out + ((size_t)t * nq + h) * hd + d0) = *(const uint2*)packed;
-            } else {
-                const int page = page_table[(size_t)slots[seq_of[t]] * max_pages + pos[u] / page_size];
-                *(uint2*)(k_cache + (((size_t)page * nkv + (h - nq)) * page_size + pos[u] % page_size) * hd + d0) =
-                    *(const uint2*)packed;
-            }
+        for (int e = 0; e < 4; ++e) packed[e] = hb_from_float<TQ>(a[e]);
+        if (is_q) {
+            *(uint2*)(q_out + ((size_t)t * nq + h) * hd + d0) = *(const uint2*)packed;
+        } else {
+            const int page = page_table[(size_t)slots[seq_of[t]] * max_pages + pos[u] / page_size];
+            *(uint2*)(k_cache + (((size_t)page * nkv + (h - nq)) * page_size + pos[u] % page_size) * hd + d0) =
+                *(const uint2*)packed;
         }
     }
 }
@@ -395,8 +397,8 @@ extern "C" int hb_qk_norm_rope_write(const float* qkv, int ld_qkv, const float* 
     HB_REQUIRE(heads <= 65535, "qk_norm_rope_write: too many heads for the grid");
     if (dtype == HB_BF16 && write_kv && T >= 64 && hd <= HB_TILED_HEAD_DIM && hd % 8 == 0 && ld_qkv % 4 == 0 &&
         slice_stride % 4 == 0 && ((uintptr_t)qkv & 15) == 0 &&
-        (cos_t == nullptr || rot_dims == hd) && (T + 63) / 64 <= 0x7fffffff) {
-        dim3 tiles((T + 63) / 64, heads);
+        (cos_t == nullptr || rot_dims == hd) && T <= 0x7fffffff - HB_TILED_TOKENS) {
+        dim3 tiles((T + HB_TILED_TOKENS - 1) / HB_TILED_TOKENS, heads);
         HB_REQUIRE(qkv_slices == 1 || slice_stride >= (size_t)T * ld_qkv, "qk_norm_rope_write: slices overlap");
 #define TILED_GO(QSV)                                                                                          \
     qk_norm_rope_write_tiled_kernel<bf16, bf16, QSV><<<tiles, 256, 0, stream>>>(                              \

@@ -31,10 +31,11 @@ MASKED_COLUMNS = 64             # of an item in whose pages are places that some
 # own. Bytes that need not be read again from which the shared one ends sooner all the same, in a model's decode steps (36 layers of 32 heads of
 # 128 over 8; microseconds a layer, shared less separate): 2 answers to 8,192 and 16,384 tokens (34, 67 MB) +2.1, -3.8; 4 to 2,048 and
 # 4,096 (25, 50 MB) +1.0, -0.8; 8 to 1,024 and 2,048 (29, 59 MB) +4.3, +0.8; 16 to 1,024, 2,048 and 2,560 (63, 126, 157 MB) +6.1, +0.5, -2.4; 32
-# to 1,024 and 2,048 (130, 260 MB) +4.3, -5.2; 64 to 1,024 and 2,048 (264, 528 MB) -1.4, -25; 128 to 1,024 (533 MB) -24.
+# to 1,024 and 2,048 (130, 260 MB) +4.3, -5.2; 48 to 1,024 (197 MB) -6; 64 to 256, 512 and 1,024 (66, 132, 264 MB) +5.6, +1.0, -9.7; 96 to 512 (199 MB) -2.4; 128 to 256
+# and 512 (133, 266 MB) +5.9, -6.9.
 SAVED_BYTES = 32 << 20
-SAVED_BYTES_EACH = 5 << 20      # and these for each sequence, of SAVED_SEQUENCES at most
-SAVED_SEQUENCES = 40
+SAVED_BYTES_EACH = 6 << 20      # and these for each sequence, of SAVED_SEQUENCES at most
+SAVED_SEQUENCES = 20
 # Tokens a sequence from which a step is worth more as a prompt: its own columns fill the products by then. 24 sequences of 8, 40 and 200 new tokens behind
 # 2,000 shared ones: 28, 46, 157 us shared, 34, 38, 121 us separate; behind 1,000: 23, 40, 128 and 23, 27, 80 us. In float32 16 sequences of 8, 40 and
 # 200 behind 256: 15, 38, 135 us shared, 21, 33, 129 us separate; behind 2,000: 37, 128, 526 and 98, 146, 566 us.
