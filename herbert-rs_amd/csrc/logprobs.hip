@@ -329,6 +329,7 @@ logprob_row_kernel(const float* __restrict__ logits, int V, const int* __restric
 extern "C" int hb_token_logprobs(const float* logits, int R, int V, const int* tokens, float* chosen, float* entropy, int* ids,
                                  float* best, int top, void* stats, void* keys, hipStream_t stream) {
     HB_REQUIRE(R > 0 && V > 0 && top >= 0 && top <= MAX_TOP && top <= V, "log probabilities: bad sizes (R=%d, V=%d, top=%d)", R, V, top);
+    HB_REQUIRE(top == 0 || (ids && best), "log probabilities: no room for %d alternatives", top);
     const int chunks = (V - 1) / CHUNK + 1;
     HB_REQUIRE((long long)R * chunks <= 0x7fffffffLL, "log probabilities: too many rows for the grid");
     HB_REQUIRE(chunks == 1 || (stats && (top == 0 || keys)), "log probabilities: rows of more than %d logits need room for their chunks", CHUNK);
