@@ -35,7 +35,7 @@ struct Item {
 // Narrow ones: operands stream from memory into registers, half a page at a time, in 16 x 16 x 32 products, whose operands are 64
 // neighbouring bytes of a row; a wave has 16 or 32 columns, the waves of a tile (four, or two each of two tiles) take the pages
 // in turn and add up their results through LDS. A sequence's own rows over the pages that they see in part (CAUSAL) are
-// narrow, too, in tiles of 16 columns.
+// narrow, too, in tiles of 16 columns. In steps of short contexts a sequence is an item and its result the row's (out), nothing is joined.
 // 256 registers and 66 KB of LDS: two workgroups a CU, so that items that wait for memory and items that compute overlap.
 // 8/32 heads of 128, microseconds (join apart): 128 answers to 32,768 tokens 86 to 92 (0.75 PFLOP/s; the products are 39 % of the time and the softmax's vector
 // work 37 %, partly side by side; with 64 columns a wave 120, since registers were moved between files), 64 to 8,192 29 (108 MB at 3.7 TB/s), 48 questions
@@ -65,6 +65,8 @@ struct SharedArgs {
     const int *order, *positions, *parts;
     int nq, nkv, kvh, G;
     float c, cap;
+    bf16* out;                          // where every row is one item's: its result; else null
+    const float* sinks;
 };
 
 // A narrow item's wave: NT tiles of 16 columns from column col0 on, every phases-th page of the item from the phase-th on. With more than one
@@ -229,11 +231,25 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
         l[t] += __shfl_xor(l[t], 32, 64);
         if (marked) l[t] = -l[t];                         // (a mark: sums are not below zero)
     }
-    auto leave = [&](int t, int d) {
-        if (mine[t]) *(f32x4*)(A.partial_o + ((size_t)place[t] * A.nq + head[t]) * HD + d * 16 + 4 * g) = oacc[t][d];
+    // (factor: of a whole result, see whole)
+    auto leave = [&](int t, int d, float factor) {
+        if (!mine[t]) return;
+        if (!CAUSAL && A.out) {
+            bf16x4 b;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = (__bf16)(oacc[t][d][e] * factor);
+            *(bf16x4*)(A.out + ((size_t)token[t] * A.nq + head[t]) * HD + d * 16 + 4 * g) = b;
+        } else {
+            *(f32x4*)(A.partial_o + ((size_t)place[t] * A.nq + head[t]) * HD + d * 16 + 4 * g) = oacc[t][d];
+        }
+    };
+    auto whole = [&](int t, float top, float total) {
+        if (CAUSAL || !A.out) return 0.f;
+        if (A.sinks) total += sink_share(A.sinks[head[t]], top, A.c);
+        return total > 0.f || total != total ? 1.0f / total : 0.f;
     };
     auto leave_ml = [&](int t, float top, float total) {
-        if (mine[t] && g == 0) ((float2*)A.partial_ml)[(size_t)place[t] * A.nq + head[t]] = make_float2(top, total);
+        if (mine[t] && g == 0 && (CAUSAL || !A.out)) ((float2*)A.partial_ml)[(size_t)place[t] * A.nq + head[t]] = make_float2(top, total);
     };
     // the waves of a tile add up what they have: each the blocks that are its own (the x-th: phase x % PHASES)
     auto join = [&](auto phases_tag) {
@@ -269,6 +285,7 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
                 for (int f = 0; f < PHASES; ++f) some |= __float_as_uint(other[f].y) >> 31;
                 total = some ? -total : total;
             }
+            const float factor = whole(t, top, total);
 #pragma unroll
             for (int d = 0; d < BLOCKS; ++d) {
                 if ((t * BLOCKS + d) % PHASES != phase) continue;
@@ -281,7 +298,7 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
                     for (int e = 0; e < 4; ++e) o[e] = fmaf(other[f].x, x[e], o[e]);
                 }
                 oacc[t][d] = o;
-                leave(t, d);
+                leave(t, d, factor);
             }
             if (phase == 0) leave_ml(t, top, total);
         }
@@ -294,8 +311,9 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             leave_ml(t, m[t], l[t]);
+            const float factor = whole(t, m[t], l[t]);
 #pragma unroll
-            for (int d = 0; d < BLOCKS; ++d) leave(t, d);
+            for (int d = 0; d < BLOCKS; ++d) leave(t, d, factor);
         }
     }
 }
@@ -408,13 +426,14 @@ __global__ void __launch_bounds__(256, 2)
 attn_shared_kernel(const bf16* __restrict__ q, const bf16* __restrict__ k_cache, const bf16* __restrict__ v_cache,
                    float* __restrict__ partial_o, float* __restrict__ partial_ml, const int* __restrict__ items,
                    const int* __restrict__ order, const int* __restrict__ parts, const int* __restrict__ positions,
-                   const int* __restrict__ page_table, int max_pages, int nq, int nkv, float c, float cap) {
+                   const int* __restrict__ page_table, int max_pages, int nq, int nkv, float c, float cap, bf16* __restrict__ out,
+                   const float* __restrict__ sinks) {
     // (of the launch, not of the kernel: see the prompt kernels)
     extern __shared__ __attribute__((aligned(1024))) char shared_lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Item it(items + (size_t)(blockIdx.x / nkv) * ITEM_INTS);
     if (it.rows == 0) return;
-    const SharedArgs A = {q, k_cache, v_cache, partial_o, partial_ml, order, positions, parts, nq, nkv, (int)(blockIdx.x % nkv), nq / nkv, c, cap};
+    const SharedArgs A = {q, k_cache, v_cache, partial_o, partial_ml, order, positions, parts, nq, nkv, (int)(blockIdx.x % nkv), nq / nkv, c, cap, out, sinks};
     const int cols = it.rows * A.G;
     const int* pt = page_table + (size_t)it.slot * max_pages;
     if (cols > 64) {
@@ -719,9 +738,10 @@ attn_shared_join_kernel(const float* __restrict__ partial_o, const float* __rest
 
 // q, out [T, nq hd]; keys [pages, nkv, 64, hd], values [pages, nkv, hd, 64]; one storage type. items [n_items, 8]; order [n_rows]; part_start [n_rows + 1]: where a row's partial results begin; parts: the places of the items' rows among
 // them; partial_o [partial results, nq, hd], partial_ml [partial results, nq, 2]. max_rows: the most rows of an item;
-// causal: some rows are of one sequence (seq_of [n_rows], slots [sequences]: only then looked at). softcap 0: none; sinks [nq] or null.
+// causal: some rows are of one sequence (seq_of [n_rows], slots [sequences]: only then looked at). direct (bfloat16, not causal, items of at most 64
+// columns): every row is in one item, whose result is the row's. softcap 0: none; sinks [nq] or null.
 extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_cache, void* out, int dtype, float* partial_o,
-                              float* partial_ml, const int* items, int n_items, int max_rows, int causal, const int* order,
+                              float* partial_ml, const int* items, int n_items, int max_rows, int causal, int direct, const int* order,
                               const int* part_start, const int* parts, int n_rows, const int* positions,
                               const int* seq_of, const int* slots, const int* page_table, int max_pages, int nq, int nkv, int hd, float scale, float softcap,
                               const float* sinks, hipStream_t stream) {
@@ -737,6 +757,7 @@ extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_
         HB_REQUIRE(hd == 32 || hd == 64 || hd == 128, "shared attention: bfloat16 heads of 32, 64 or 128, not %d", hd);
         HB_REQUIRE((long long)max_rows * G <= 128, "shared attention: items of %d rows x %d heads exceed 128 columns", max_rows, G);
         HB_REQUIRE((long long)n_items * nkv <= 0x7fffffffLL, "shared attention: too many items for the grid");
+        HB_REQUIRE(!direct || (!causal && (long long)max_rows * G <= 64), "shared attention: items that are whole rows' have at most 64 columns, a token a sequence");
         const float c = scale * 1.4426950408889634f, cap = softcap > 0.f ? softcap / scale : 0.f;
         const Spoiled spoiled = {(const bf16*)v_cache, positions, seq_of, slots, page_table, max_pages, nkv};
         const dim3 grid((unsigned)(n_items * nkv));
@@ -748,9 +769,9 @@ extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_
             HB_REQUIRE(allowed == hipSuccess, "shared attention: %d bytes of LDS refused: %s", lds, hipGetErrorString(allowed)); \
             attn_shared_kernel<HD, CAUSAL><<<grid, 256, lds, stream>>>(                                                      \
                 (const bf16*)q, (const bf16*)k_cache, (const bf16*)v_cache, partial_o, partial_ml, items, order, parts, positions, \
-                page_table, max_pages, nq, nkv, c, cap);                                                                     \
+                page_table, max_pages, nq, nkv, c, cap, direct ? (bf16*)out : nullptr, sinks);                               \
             HB_CHECK_LAUNCH("shared attention");                                                                             \
-            attn_shared_join_kernel<bf16, HD / 4, CAUSAL><<<join(HD / 4), 256, 0, stream>>>(partial_o, partial_ml, (bf16*)out, order,     \
+            if (!direct) attn_shared_join_kernel<bf16, HD / 4, CAUSAL><<<join(HD / 4), 256, 0, stream>>>(partial_o, partial_ml, (bf16*)out, order,     \
                                                                                part_start, n_rows, nq, hd, c, sinks, spoiled); \
         }
 #define HB_SHARED(HD)                                                                                                        \
@@ -764,6 +785,7 @@ extern "C" int hb_attn_shared(const void* q, const void* k_cache, const void* v_
 #undef HB_SHARED
 #undef HB_SHARED_KERNEL
     } else if (dtype == HB_F32) {
+        HB_REQUIRE(!direct, "shared attention: float32 items leave parts of rows");
         HB_REQUIRE(hd > 0 && hd <= 256 && hd % 4 == 0, "shared attention: float32 heads of up to 256 entries in whole quads, not %d", hd);
         const long long col_tiles = ((long long)max_rows * G + 15) / 16;
         HB_REQUIRE((long long)n_items * nkv * col_tiles <= 0x7fffffffLL, "shared attention: too many items for the grid");

@@ -8,6 +8,7 @@ import ctypes
 import numpy as np
 import torch
 
+from ..cache import SharedPages
 from ..errors import BackendError
 from ..hosted import send, send_into
 from . import lib, mfma, ops
@@ -15,7 +16,7 @@ from .ops import _stream
 
 _P, _I, _F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
 lib.register_signatures("attention_shared", {
-    "hb_attn_shared": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P],
+    "hb_attn_shared": [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _P, _P, _P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _F, _F, _P, _P],
 })
 
 ITEM_INTS = 8
@@ -27,6 +28,9 @@ F32_MOST_DIM = 256
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
 OPERANDS = ("q", "out", "key pages", "value pages", "page_table", "positions", "seq_of", "slots", "sinks")
 MASKED_COLUMNS = 64             # of an item in whose pages are places that some of its rows see and others do not: the wide ones ask no mask
+# Pages of the longest sequence up to which every sequence is an item of its own, a page a wave, and nothing is joined: of 4 pages 8.2 us and not 9.9 to 12.6 (2 to
+# 32 sequences, 2 to 8 kv heads of 128), 64 sequences of 8 heads 12.4 and 15.4; of 8 pages 11.7 and 10.8 to 13.4, 64 sequences 19.7 and 16.9.
+BY_ITSELF_PAGES = 4
 # The attention of one sequence after another also normalizes, rotates and writes what the projection gave; before the shared one that is a kernel of its
 # own. Bytes that need not be read again from which the shared one ends sooner all the same, in a model's decode steps (36 layers of 32 heads of
 # 128 over 8; microseconds a layer, shared less separate): 2 answers to 8,192 and 16,384 tokens (34, 67 MB) +2.1, -3.8; 4 to 2,048 and
@@ -121,15 +125,26 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
     return as32(items), as32(order), as32(part_start), as32(parts), most
 
 
+def _by_itself(meta, nkv, dtype):
+    """True for steps of short contexts, which end sooner without a second kernel: every sequence is an item, whose result is the row's."""
+    return (dtype == torch.bfloat16 and meta.max_new == 1 and meta.num_seqs * nkv <= WORKGROUPS[dtype]
+            and int(meta.host_context.max()) <= 64 * BY_ITSELF_PAGES)
+
+
 def _planned(meta, group, nkv, dtype, grid=1):
-    return plan(meta.host_starts, meta.host_context, meta.host_slots, meta.shared, group, nkv, COLUMNS[dtype], WORKGROUPS[dtype], grid)
+    """(What `plan` gives, whether every row is one item's.)"""
+    sharing, workgroups, direct = meta.shared, WORKGROUPS[dtype], _by_itself(meta, nkv, dtype)
+    if direct:
+        n = len(sharing.order)
+        sharing, workgroups = SharedPages(np.arange(n), [(i, 1, 0, -1) for i in range(n)]), 1
+    return (*plan(meta.host_starts, meta.host_context, meta.host_slots, sharing, group, nkv, COLUMNS[dtype], workgroups, grid), direct)
 
 
 class Plan:
     """A plan on the GPU: of meta.shared as it is now."""
 
     def __init__(self, meta, group, nkv, dtype):
-        items, order, part_start, parts, self.max_rows = _planned(meta, group, nkv, dtype)
+        items, order, part_start, parts, self.max_rows, self.direct = _planned(meta, group, nkv, dtype)
         both = send(np.concatenate([a.ravel() for a in (items, order, part_start, parts)]), meta.positions.device)
         at = np.cumsum([a.size for a in (items, order, part_start, parts)])
         self.items, self.order, self.part_start, self.parts = both[:at[0]], both[at[0]:at[1]], both[at[1]:at[2]], both[at[2]:]
@@ -138,13 +153,13 @@ class Plan:
 
 class StaticPlan:
     """The plans of decode steps of one batch size, in buffers that stay where they are while they are large enough: a recorded
-    graph reads them. `shape` is what such a graph is tied to: which buffers, how many workgroups (in steps of GRID) and how much room
-    for partial results (powers of two)."""
+    graph reads them. `shape` is what such a graph is tied to: which buffers, how many workgroups (in steps of GRID), how much room
+    for partial results (powers of two), and whether there are any."""
     GRID = 16
 
     def __init__(self, group, nkv, dtype, rows, device):
         self.group, self.nkv, self.dtype, self.rows, self.device = group, nkv, dtype, rows, device
-        self.max_rows = max(1, COLUMNS[dtype] // group)
+        self.direct = False
         self.made = 0               # buffers so far: those that were outgrown are kept, a graph may hold their addresses
         self._outgrown = []
         self._buffer, self._rooms, self._filled_for = None, (0, 0), None
@@ -152,7 +167,11 @@ class StaticPlan:
 
     @property
     def shape(self):
-        return self.made, self.n_items, self.n_parts
+        return self.made, self.n_items, self.n_parts, self.direct
+
+    @property
+    def max_rows(self):
+        return 1 if self.direct else max(1, COLUMNS[self.dtype] // self.group)
 
     def refill(self, meta):
         """Work the step's plan out and send it, unless it is that of the step before (it changes where a sequence begins a page)."""
@@ -160,7 +179,7 @@ class StaticPlan:
         before = self._filled_for
         if before is not None and before[0] is meta.shared and before[1:] == filled_for[1:]:
             return
-        items, order, part_start, parts, _ = _planned(meta, self.group, self.nkv, self.dtype, self.GRID)
+        items, order, part_start, parts, _, self.direct = _planned(meta, self.group, self.nkv, self.dtype, self.GRID)
         self.n_items, self.n_parts = len(items), 1 << (len(parts) - 1).bit_length()
         if len(items) > self._rooms[0] or len(parts) > self._rooms[1]:
             if self._buffer is not None:
@@ -232,10 +251,12 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
     if meta.max_context > 64 * table.shape[1]:
         raise BackendError(f"shared attention: a context of {meta.max_context} tokens does not fit a table of {table.shape[1]} pages")
     p = _plan_of(meta, nq, nkv, hd, q.dtype)
-    if scratch is None:
+    if p.direct:
+        po = pml = None
+    elif scratch is None:
         po, pml = (torch.empty(p.n_parts * nq * n, dtype=torch.float32, device=q.device) for n in (hd, 2))
     else:
         po, pml = mfma._partial_buffers(scratch, q.device, p.n_parts * nq, 1, hd)
     lib.call("attention_shared", "hb_attn_shared", q, keys, values, out, ops.dtype_code(q), po, pml, p.items, p.n_items, p.max_rows,
-             1 if meta.max_new > 1 else 0, p.order, p.part_start, p.parts, T, meta.positions, meta.seq_of, meta.slots, table, table.shape[1],
+             1 if meta.max_new > 1 else 0, 1 if p.direct else 0, p.order, p.part_start, p.parts, T, meta.positions, meta.seq_of, meta.slots, table, table.shape[1],
              nq, nkv, hd, float(scale), float(softcap or 0.0), sinks, _stream())

@@ -151,7 +151,7 @@ def test_what_the_shared_attention_refuses():
 
 
 def call(**changed):
-    args = dict(q=None, k=None, v=None, out=None, dtype=1, po=None, pml=None, items=None, n_items=1, max_rows=1, causal=0, order=None, start=None,
+    args = dict(q=None, k=None, v=None, out=None, dtype=1, po=None, pml=None, items=None, n_items=1, max_rows=1, causal=0, direct=0, order=None, start=None,
                 parts=None, n_rows=1, positions=None, seq_of=None, slots=None, table=None, max_pages=1, nq=4, nkv=2, hd=64, scale=0.1, softcap=0.0,
                 sinks=None, stream=None)
     args.update(changed)
@@ -163,7 +163,8 @@ def call(**changed):
     ({"max_rows": 65}, "exceed 128 columns"), ({"scale": 0.0}, "positive"), ({"softcap": -1.0}, "positive"),
     ({"scale": float("nan")}, "positive"), ({"n_rows": 1 << 30}, "exceed|too many rows"), ({"n_items": 1 << 30}, "too many items"),
     ({"dtype": 0, "hd": 62}, "whole quads"), ({"dtype": 0, "hd": 260}, "up to 256"), ({"dtype": 0, "k": 8}, "16-byte"), ({"q": 2}, "16-byte"), ({"v": 24}, "16-byte"),
-    ({"dtype": 0, "n_items": 1 << 30}, "too many items")])
+    ({"dtype": 0, "n_items": 1 << 30}, "too many items"), ({"dtype": 0, "direct": 1}, "parts of rows"), ({"direct": 1, "causal": 1}, "whole rows"),
+    ({"direct": 1, "max_rows": 33}, "whole rows")])
 def test_calls_that_the_entry_refuses(changed, text):
     with pytest.raises(BackendError, match=text):
         call(**changed)

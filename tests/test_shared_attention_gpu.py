@@ -33,10 +33,18 @@ def run(seqs, held, news, nq, nkv, hd, dtype, seed=0, sinks=None, softcap=None, 
     assert meta.shared is not None
     q, kv = inputs(table, pages, sum(news), nq, nkv, hd, dtype, seed, dev())
     out = torch.full_like(q, float("nan"))
-    shared.attention(q, meta, kv, out, nq, nkv, hd, hd ** -0.5, sinks=sinks, softcap=softcap)
-    if check:
-        want = reference(q, kv, table, held, news, nq, nkv, hd, hd ** -0.5, sinks, softcap)
-        compare(out, want, dtype, hd, max(h + n for h, n in zip(held, news)), "bf16" if dtype == torch.bfloat16 else "f32")
+    want = reference(q, kv, table, held, news, nq, nkv, hd, hd ** -0.5, sinks, softcap) if check else None
+    for whole_rows in ((True, False) if dtype == BF and max(news) == 1 else (False,)):       # (short contexts have another form)
+        limit = shared.BY_ITSELF_PAGES
+        shared.BY_ITSELF_PAGES = 1 << 20 if whole_rows else 0
+        try:
+            meta.derived.clear()
+            shared.attention(q, meta, kv, out.fill_(float("nan")), nq, nkv, hd, hd ** -0.5, sinks=sinks, softcap=softcap)
+        finally:
+            shared.BY_ITSELF_PAGES = limit
+        assert next(v for k, v in meta.derived.items() if k[0] == "shared_plan").direct == (whole_rows and len(held) * nkv <= 512)
+        if check:
+            compare(out, want, dtype, hd, max(h + n for h, n in zip(held, news)), "bf16" if dtype == torch.bfloat16 else "f32")
     return q, meta, kv, out, table
 
 
