@@ -93,15 +93,15 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
     bf16x8 ka[DEPTH][2][STEPS], va[DEPTH][BLOCKS], qreg[NT][STEPS];
     const int k_lane = (8 * (c16 >> 2) + (c16 & 3)) * HD + g * 8, v_lane = c16 * PAGE + g * 8;
     // (h: half of a page, 2 x its place among the item's pages + which)
-    auto load_keys = [&](int h, bf16x8 (&k)[2][STEPS]) {
-        const bf16* kp = A.k_cache + ((size_t)pt[it.page0 + (h >> 1)] * A.nkv + A.kvh) * STAGE + (h & 1) * 32 * HD + k_lane;
+    auto load_keys = [&](int page, int h, bf16x8 (&k)[2][STEPS]) {
+        const bf16* kp = A.k_cache + ((size_t)page * A.nkv + A.kvh) * STAGE + (h & 1) * 32 * HD + k_lane;
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int s = 0; s < STEPS; ++s) k[b][s] = *(const bf16x8*)(kp + b * 4 * HD + s * 32);
     };
-    auto load_values = [&](int h, bf16x8 (&v)[BLOCKS]) {
-        const bf16* vp = A.v_cache + ((size_t)pt[it.page0 + (h >> 1)] * A.nkv + A.kvh) * STAGE + (h & 1) * 32 + v_lane;
+    auto load_values = [&](int page, int h, bf16x8 (&v)[BLOCKS]) {
+        const bf16* vp = A.v_cache + ((size_t)page * A.nkv + A.kvh) * STAGE + (h & 1) * 32 + v_lane;
 #pragma unroll
         for (int d = 0; d < BLOCKS; ++d) v[d] = *(const bf16x8*)(vp + d * 16 * PAGE);
     };
@@ -109,11 +109,12 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
     auto next = [&](int h) { return (h & 1) ? h + 2 * phases - 1 : h + 1; };      // this wave's next half
     int h = 2 * phase;
     if (h < halves) {                                     // (a page is two halves: the second is there too)
-        load_keys(h, ka[0]);
-        load_values(h, va[0]);
+        const int page = pt[it.page0 + phase];
+        load_keys(page, h, ka[0]);
+        load_values(page, h, va[0]);
         if constexpr (DEPTH == 2) {
-            load_keys(h + 1, ka[1]);
-            load_values(h + 1, va[1]);
+            load_keys(page, h + 1, ka[1]);
+            load_values(page, h + 1, va[1]);
         }
     }
 #pragma unroll
@@ -143,9 +144,10 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
 #pragma unroll
         for (int d = 0; d < BLOCKS; ++d) oacc[t][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
-    auto half = [&](bf16x8 (&k)[2][STEPS], bf16x8 (&v)[BLOCKS]) {
+    auto half = [&](auto more_tag, bf16x8 (&k)[2][STEPS], bf16x8 (&v)[BLOCKS]) {
+        constexpr bool MORE = decltype(more_tag)::value;  // there is a half whose operands take these registers next
         const int key0 = it.page0 * PAGE + h * 32;
-        const int following = DEPTH == 2 ? h + 2 * phases : next(h);     // the half whose operands take these registers next
+        const int following = DEPTH == 2 ? h + 2 * phases : next(h), page = MORE ? pt[it.page0 + (following >> 1)] : 0;
         f32x4 st[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t)
@@ -156,7 +158,7 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
                 for (int s = 0; s < STEPS; ++s) st[t][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[b][s], qreg[t][s], st[t][b], 0, 0, 0);
             }
         __builtin_amdgcn_sched_barrier(0);
-        if (following < halves) load_keys(following, k);
+        if (MORE) load_keys(page, following, k);
         __builtin_amdgcn_sched_barrier(0);
         bf16x8 pb[NT];
 #pragma unroll
@@ -216,13 +218,21 @@ __device__ __forceinline__ void narrow_item(const SharedArgs& A, const Item& it,
             for (int t = 0; t < NT; ++t) oacc[t][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(clean, pb[t], oacc[t][d], 0, 0, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
-        if (following < halves) load_values(following, v);
+        if (MORE) load_values(page, following, v);
         __builtin_amdgcn_sched_barrier(0);
         h = next(h);
     };
-    while (h < halves) {
-        half(ka[0], va[0]);
-        if constexpr (DEPTH == 2) half(ka[1], va[1]);
+    // Within the loop every load is issued, whatever the item: the compiler counts what is in flight, and waits for all of it where it cannot.
+    __builtin_amdgcn_s_waitcnt(0x0f70);                   // (no load is left: of the queries, that is, which the loop then need not wait for)
+    if (h < halves) {
+        const std::true_type more;
+        const std::false_type last;
+        while ((DEPTH == 2 ? h + 2 * phases : next(h)) < halves) {
+            half(more, ka[0], va[0]);
+            if constexpr (DEPTH == 2) half(more, ka[1], va[1]);
+        }
+        half(last, ka[0], va[0]);
+        if constexpr (DEPTH == 2) half(last, ka[1], va[1]);
     }
     const bool marked = CAUSAL && __builtin_amdgcn_ballot_w64(odd != 0) != 0;
 #pragma unroll

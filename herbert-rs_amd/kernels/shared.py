@@ -28,9 +28,10 @@ F32_MOST_DIM = 256
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
 OPERANDS = ("q", "out", "key pages", "value pages", "page_table", "positions", "seq_of", "slots", "sinks")
 MASKED_COLUMNS = 64             # of an item in whose pages are places that some of its rows see and others do not: the wide ones ask no mask
-# Pages of the longest sequence up to which every sequence is an item of its own, a page a wave, and nothing is joined: of 4 pages 8.2 us and not 9.9 to 12.6 (2 to
-# 32 sequences, 2 to 8 kv heads of 128), 64 sequences of 8 heads 12.4 and 15.4; of 8 pages 11.7 and 10.8 to 13.4, 64 sequences 19.7 and 16.9.
-BY_ITSELF_PAGES = 4
+# Pages of the longest sequence up to which every sequence is an item of its own, whose pages four waves of one CU read (at 40 bytes a nanosecond), and nothing
+# is joined. 2, 8 and 64 sequences of 4, 8 and 8 kv heads of 128: of 4 pages 8.0, 8.1, 12.0 us by themselves, 10.1, 11.3, 15.3 joined; of 6 9.2, 9.4, 15.5 and 11.0, 11.8,
+# 15.9; of 8 10.5, 10.8, 18.5 and 10.9, 11.8, 16.6.
+BY_ITSELF_PAGES = 6
 # The attention of one sequence after another also normalizes, rotates and writes what the projection gave; before the shared one that is a kernel of its
 # own. Bytes that need not be read again from which the shared one ends sooner all the same, in a model's decode steps (36 layers of 32 heads of
 # 128 over 8; microseconds a layer, shared less separate): 2 answers to 8,192 and 16,384 tokens (34, 67 MB) +2.1, -3.8; 4 to 2,048 and
