@@ -188,9 +188,9 @@ __device__ __forceinline__ void leave_top(const Row& r, uint64_t key, int* id, f
 }
 
 // stats [row][chunk]: (m, S, T); keys [row][rank][chunk], so that neighbours are alike in rank. One chunk a row: the row's results themselves.
-// (eight waves a SIMD: all 38 chunks of 54 rows of 151,936 at a time)
+// (seven waves a SIMD hold the registers; eight, with one of them in memory, take as long)
 template <bool TOP>
-__global__ void __launch_bounds__(THREADS, 8)
+__global__ void __launch_bounds__(THREADS, 7)
 logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restrict__ tokens, float* __restrict__ chosen,
                      float* __restrict__ entropy, int* __restrict__ ids, float* __restrict__ best, int top, int chunks,
                      float4* __restrict__ stats, uint64_t* __restrict__ keys) {
@@ -253,9 +253,14 @@ logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restr
         const uint64_t largest = id_at(which) < len ? key_of(mine, first + id_at(which)) : (uint64_t)0;
         select_top(sh, top, largest, [&](uint64_t bound, auto f) {
             const float least = bound > 1 ? value_of(bound) : -INFINITY;
+            if (mine >= least) f(largest);
+            int n = 0;                                    // (few threads have a second one)
 #pragma unroll
-            for (int i = 0; i < PER; ++i)
-                if (x[i] >= least) f(id_at(i) < len ? key_of(x[i], first + id_at(i)) : (uint64_t)0);
+            for (int i = 0; i < PER; ++i) n += x[i] >= least ? 1 : 0;
+            if (n > 1)
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    if (x[i] >= least && i != which) f(id_at(i) < len ? key_of(x[i], first + id_at(i)) : (uint64_t)0);
         }, [&](uint64_t bound) {
             // (a bound need not be a logit's key: below all of them, and between those of -0, of which there are none, and 0)
             const uint64_t lowest = (uint64_t)0x007fffffu << 32, zero = (uint64_t)0x80000000u << 32;
