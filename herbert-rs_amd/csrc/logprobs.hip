@@ -53,6 +53,9 @@ __device__ __forceinline__ uint64_t shfl_xor_u64(uint64_t v, int off) {
     return ((uint64_t)hi << 32) | lo;
 }
 
+// How many of the wave's lanes say so.
+__device__ __forceinline__ int in_wave(bool is) { return __popcll(__builtin_amdgcn_ballot_w64(is)); }
+
 struct Selecting {
     uint64_t list[LISTED], last[RANKED];
     uint64_t groups[64];
@@ -60,19 +63,16 @@ struct Selecting {
 };
 
 // A bound from which there are `most` keys or fewer, but `top` at least: between lo, from which there are `count`, and hi, from which there
-// are fewer than `top`, by halving. of(bound): how many of the thread's keys lie at or above a bound.
+// are fewer than `top`, by halving. of(bound): how many of the wave's keys lie at or above a bound.
 template <class Of>
 __device__ uint64_t narrowed(Selecting& sh, int top, int most, uint64_t lo, uint64_t hi, int count, Of of) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    while (count > most && hi - lo > 1) {
+    for (int turn = 0; count > most && hi - lo > 1; turn ^= 1) {      // (two places in turn: one barrier)
         const uint64_t mid = lo + (hi - lo) / 2;
         int n = of(mid);
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
-        if (lane == 0) sh.above[wave][0] = n;
+        if (lane == 0) sh.above[wave][turn] = n;
         __syncthreads();
-        n = (sh.above[0][0] + sh.above[1][0]) + (sh.above[2][0] + sh.above[3][0]);
-        __syncthreads();
+        n = (sh.above[0][turn] + sh.above[1][turn]) + (sh.above[2][turn] + sh.above[3][turn]);
         if (n >= top) {
             lo = mid;
             count = n;
@@ -85,7 +85,7 @@ __device__ uint64_t narrowed(Selecting& sh, int top, int most, uint64_t lo, uint
 
 // The `top` largest of the keys that a workgroup holds, written by put(rank, key): ranks 0 .. top - 1, those that there is no key
 // for with the key 0. largest: the thread's own largest key; each(bound, f) hands f the thread's keys from bound on, and may hand it others;
-// counted(bound): how many they are.
+// counted(bound): how many the wave's are.
 // The n-th largest of the 64 largest keys of four threads each bounds the n largest of all from below. The keys at or above it are listed,
 // mostly few; where they are many, the bound is moved up by halving first (an order of the keys in memory that puts the largest side by side
 // leaves up to 16 for each of them). The last ones are ranked by counting.
@@ -140,7 +140,7 @@ __device__ void select_top(Selecting& sh, int top, uint64_t largest, Each each, 
         if (listed)
             bound = narrowed(sh, top, RANKED, bound, hi, n, [&](uint64_t from) {
                 int c = 0;
-                of_list([&](uint64_t key) { c += key >= from ? 1 : 0; });
+                for (int i = tid; i - tid < n; i += THREADS) c += in_wave(i < n && sh.list[i] >= from);
                 return c;
             });
         else
@@ -269,7 +269,7 @@ logprob_chunk_kernel(const float* __restrict__ logits, int V, const int* __restr
             const int last = (int)min(~(uint32_t)bound, (uint32_t)(first + len - 1)) - first;
             int n = 0;
 #pragma unroll
-            for (int i = 0; i < PER; ++i) n += (x[i] > least || (x[i] == least && id_at(i) <= last)) ? 1 : 0;
+            for (int i = 0; i < PER; ++i) n += in_wave(x[i] > least || (x[i] == least && id_at(i) <= last));
             return n;
         }, [&](int rank, uint64_t key) {
             if (chunks > 1) keys[(r * top + rank) * chunks + chunk] = key;
@@ -323,7 +323,7 @@ logprob_row_kernel(const float* __restrict__ logits, int V, const int* __restric
             for (int i = tid; i < n; i += THREADS) f(keys[i]);
         }, [&](uint64_t bound) {
             int c = 0;
-            for (int i = tid; i < n; i += THREADS) c += keys[i] >= bound ? 1 : 0;
+            for (int i = tid; i - tid < n; i += THREADS) c += in_wave(i < n && keys[i] >= bound);
             return c;
         }, [&](int rank, uint64_t key) { leave_top(whole, key, ids + r * top + rank, best + r * top + rank); });
     }
