@@ -7,8 +7,8 @@
 // registers (16 a thread), finds its (m, S, T) and its own `top` largest; a second kernel adds a row's chunks up:
 //   S = sum S_c e^(m_c - m),   T = sum (T_c + (m_c - m) S_c) e^(m_c - m).
 // A row of one chunk needs no second kernel.
-// 2,048 rows of 151,936 in 201 to 213 us, 6.1 TB/s: HBM. With alternatives by instructions: 64 rows and 20 of them 15 us for the chunks (39 MB; about 550 instructions a wave, a
-// third of them alternatives; of 8,192 logits a chunk as long, and one row 6.5 instead of 5.6), 5 us for the rows; one row 5.6 and 3.8, the least that two kernels take.
+// 2,048 rows of 151,936 in 201 to 213 us, 6.1 TB/s: HBM. With alternatives by instructions: 64 rows and 20 of them 14.4 us for the chunks (39 MB; about 520 instructions a wave, a
+// quarter of them alternatives; chunks of 8,192 took as long for 64 rows and 0.9 us more for one), 5 us for the rows; one row 5.2 and 4.0, near the least that two kernels take.
 // The reference computes a softmax on the host to draw a token (crates/core/src/sampler.rs:72-145) and reports no
 // probabilities.
 #include "common.h"

@@ -24,6 +24,7 @@ def used(monkeypatch):
     calls = []
     monkeypatch.setattr(shared, "SAVED_BYTES", 1)
     monkeypatch.setattr(shared, "SAVED_BYTES_EACH", 0)
+    monkeypatch.setattr(shared, "BY_ITSELF_PAGES", 0)
     monkeypatch.setattr(shared, "MANY_TOKENS", {torch.bfloat16: 1000, torch.float32: 1000})
     real = shared.attention
 
@@ -73,6 +74,75 @@ def test_forks_go_on_as_if_each_had_had_the_prompt(name, dtype, graphs, used, mo
         engine.free_slot(slots[i])
     engine.cache.check()
     assert all(g.pages.held_count == 0 for g in engine.cache.kv_groups.values())
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_steps_pass_from_whole_rows_to_joined_ones(dtype, used, model_root, monkeypatch):
+    """Contexts grow over the length up to which sequences are items of their own, through recorded steps, while slots end, are forked anew and
+    the batch passes through several sizes; then back to short ones."""
+    monkeypatch.setattr(shared, "BY_ITSELF_PAGES", 3)
+    folder, vocab = make_folder(model_root, "D", dtype), CONFIGS["D"][0]["vocab_size"]
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 60)
+    for prompt_length in (180, 90):
+        texts = {}
+        first = engine.alloc_slot()
+        texts[first] = random_tokens(vocab, prompt_length, prompt_length)
+        engine.step([StepEntry(first, texts[first], [])])
+        for new in engine.fork(first, 6):
+            texts[new] = list(texts[first])
+        for at in range(26):
+            if at in (5, 13, 20):
+                gone = sorted(texts)[at % len(texts)]
+                engine.free_slot(gone)
+                del texts[gone]
+            if at == 16:
+                source = sorted(texts)[0]
+                for new in engine.fork(source, 3):
+                    texts[new] = list(texts[source])
+            for s in texts:
+                texts[s] = texts[s] + random_tokens(vocab, 1, 100 * at + s)
+            rows = engine.step([StepEntry(s, t[-1:], [0]) for s, t in texts.items()]).cpu().numpy()
+            if at % 5 == 0 or at in (12, 13, 14, 17):
+                for (s, t), row in zip(texts.items(), rows):
+                    ok, err = close(row, plain_logits(folder, t)[-1], dtype, "D", "growing forks")
+                    assert ok, f"step {at}, slot {s}: {err}"
+        for s in texts:
+            engine.free_slot(s)
+    engine.cache.check()
+    assert len(used) >= 3
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_two_engines_on_two_streams_decode_their_forks_at_once(dtype, used, model_root):
+    folder, vocab = make_folder(model_root, "D", dtype), CONFIGS["D"][0]["vocab_size"]
+    prompts = [random_tokens(vocab, 150, 1), random_tokens(vocab, 200, 2)]
+    tokens = torch.tensor(random_tokens(vocab, 20 * 4, 3), dtype=torch.int32, device="cuda").view(20, 4)
+
+    def begin(prompt):
+        engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 30)
+        slot = engine.alloc_slot()
+        engine.step([StepEntry(slot, prompt, [])])
+        return engine, [slot] + engine.fork(slot, 3)
+
+    def one(engine, slots, i):
+        return engine.step([StepEntry(s, [0], [0]) for s in slots], tokens_on_device=tokens[i])
+    want = []
+    for prompt in prompts:
+        engine, slots = begin(prompt)
+        want.append([one(engine, slots, i) for i in range(20)])
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    made = []
+    for prompt, side in zip(prompts, sides):
+        with torch.cuda.stream(side):
+            made.append(begin(prompt))
+    got = [[], []]
+    for i in range(20):
+        for k, side in enumerate(sides):
+            with torch.cuda.stream(side):
+                got[k].append(one(*made[k], i))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for k in range(2) for a, b in zip(got[k], want[k]))
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
