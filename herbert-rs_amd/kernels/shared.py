@@ -76,11 +76,14 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
     if len(sharing.order) != len(counts):
         raise BackendError(f"shared attention: pages shared by {len(sharing.order)} sequences in a step of {len(counts)}")
     row_of = np.concatenate([[0], np.cumsum(counts[sharing.order])])            # a sequence's first row in the order
-    order = np.concatenate([np.arange(starts[i], starts[i + 1]) for i in sharing.order])
+    of_row = np.repeat(sharing.order, counts[sharing.order])                    # whose row it is
+    order = starts[of_row] + np.arange(len(of_row)) - row_of[np.repeat(np.arange(len(counts)), counts[sharing.order])]
     tall = max(1, columns // group)
     short = max(1, MASKED_COLUMNS // group) if columns == 128 else tall
     tiles = []                                                                  # row0, rows, sequence, first page, end, first page seen in part
-    for first, count, page, end in sharing.nodes:
+    nodes = np.array(sharing.nodes, dtype=np.int64).reshape(-1, 4)
+    alone = (nodes[:, 3] < 0) & (counts[sharing.order[nodes[:, 0]]] == 1)       # a sequence's own pages, one row: all of them at once
+    for first, count, page, end in nodes[~alone].tolist():
         a, b, seq = int(row_of[first]), int(row_of[first + count]), int(sharing.order[first])
         for r, n in _even(a, b, tall):
             if end >= 0:
@@ -94,14 +97,17 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
             for u, m in _even(r, r + n, short):
                 first_seen, last_seen = int(context[seq]) - (b - u), int(context[seq]) - (b - (u + m)) - 1
                 tiles.append((u, m, seq, page_from, last_seen // 64 + 1, first_seen // 64))
-    row0, rows, seq, page, end, whole = np.array(tiles, dtype=np.int64).T
+    first = nodes[alone, 0]
+    seen = (context[sharing.order[first]] - 1) // 64
+    of_one = np.stack([row_of[first], np.ones_like(first), sharing.order[first], nodes[alone, 2], seen + 1, seen])
+    row0, rows, seq, page, end, whole = np.concatenate([np.array(tiles, dtype=np.int64).reshape(-1, 6).T, of_one], axis=1)
     cols, pages = rows * group, end - page
     turns = np.where(cols <= 32, 4, np.where(cols <= 64, 2, 1)) if columns == 128 else np.ones_like(cols)
     share = max(1, -(-int(pages.sum()) * nkv // workgroups))
     per = -(-share // turns) * turns
     ranges = -(-pages // per)
     per = -(-(-(-pages // ranges)) // turns) * turns
-    of = np.repeat(np.arange(len(tiles)), ranges)
+    of = np.repeat(np.arange(len(rows)), ranges)
     nth = np.arange(len(of)) - np.repeat(np.cumsum(ranges) - ranges, ranges)
     items = np.zeros((len(of), ITEM_INTS), dtype=np.int64)
     items[:, 0], items[:, 1], items[:, 2] = row0[of], rows[of], np.asarray(slots, dtype=np.int64)[seq[of]]
