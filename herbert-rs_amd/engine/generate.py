@@ -141,8 +141,10 @@ class Generator:
         eng = self.engine
         spec = eng.spec
         capacity = eng.cache.n_pages * PAGE_TOKENS
-        batches = plan_batches([len(p) for p in prompts], params.max_tokens, self.max_batch,
-                               capacity, spec.max_positions, params.samples)
+        # (further answers to a prompt may need no page of their own, but every one a slot)
+        at_once = min(self.max_batch, max(1, eng.cache.slots.free_count))
+        batches = plan_batches([len(p) for p in prompts], params.max_tokens, at_once, capacity,
+                               spec.max_positions, params.samples)
         prompts = [p for p in prompts for _ in range(params.samples)]
         chooser = self.make_chooser(params, len(prompts), spec.vocab_size, eng.device)
         results = [None] * len(prompts)

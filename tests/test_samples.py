@@ -125,3 +125,24 @@ def test_the_books_of_free_slots_hold():
     run([[5]], 4, engine=engine, max_tokens=2)
     slots.check()
     assert slots.held_count == 0
+
+
+@pytest.mark.parametrize("chunk", [None, 2])
+@pytest.mark.parametrize("slots, held", [(2, 0), (1, 0), (4, 2)])
+def test_answers_run_in_as_many_batches_as_there_are_slots_for(slots, held, chunk):
+    """More answers than free slots; a prompt of as many positions as the model has, whose further answers need no page of their own."""
+    engine = ForkingEngine()
+    engine.cache.slots = FreeList(slots, "slot")
+    mine = [engine.alloc_slot() for _ in range(held)]
+    prompts = [[5, 6, 7], [20]]
+    _, gen, results = run(prompts, 5, engine=engine, chunk=chunk, max_tokens=4)
+    assert [r.tokens for r in results] == [want(prompts[i // 5], i, 4) for i in range(10)]
+    assert gen.stats.batches == 10 // (slots - held)
+    assert engine.cache.slots.held_count == held
+    engine.spec.max_positions = 64
+    full = [3] * 64
+    _, _, results = run([full], 5, engine=engine, chunk=chunk, max_tokens=4)
+    assert [(r.tokens, r.stop_reason) for r in results] == [(want(full, i, 1), "length") for i in range(5)]
+    for s in mine:
+        engine.free_slot(s)
+    assert engine.cache.slots.held_count == 0
