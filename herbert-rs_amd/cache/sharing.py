@@ -4,6 +4,7 @@ Slots that were forked from one another name the same pages at the beginning of 
 a cache a sequence (crates/backends/backend_common/src/kv_cache.rs:270-273) and shares nothing.
 """
 from dataclasses import dataclass, field
+from functools import cached_property
 from typing import List, Tuple
 
 import numpy as np
@@ -32,7 +33,7 @@ class SharedPages:
             self._filled = SharedPages(np.concatenate([self.order, np.array(more, dtype=np.int64)]), self.nodes + [(i, 1, 0, -1) for i in more])
         return self._filled
 
-    @property
+    @cached_property
     def pages_saved(self):
         """How many pages fewer are read than if every sequence read its own."""
         return sum((count - 1) * (end - page) for _, count, page, end in self.nodes if count > 1)

@@ -192,8 +192,10 @@ class StaticDecodeMeta:
 
     RANGE_LISTS = 4      # lists of ranges (BatchMeta.ranges_for) that the buffers have room for
 
-    def __init__(self, batch_size, device, pad_slot=0):
+    def __init__(self, batch_size, device, pad_slot=0, worth=None):
+        """worth: a function of the meta that says of each kind of cache whether reading shared pages together pays (kernels.shared.worth_over)."""
         B = self.batch_size = batch_size
+        self.worth = worth
         self.pad_slot = int(pad_slot)
         size = 7 * B + 1 + self.RANGE_LISTS * (B + 2)
         self.host = torch.zeros(size, dtype=torch.int32, pin_memory=torch.device(device).type == "cuda")
@@ -229,11 +231,12 @@ class StaticDecodeMeta:
 
     @property
     def shared_shape(self):
-        """What a recorded step with shared pages is tied to beside its batch size and contexts; None where no pages are shared to
-        any use."""
+        """What a recorded step with shared pages is tied to beside its batch size and contexts: over which caches it pays, and the
+        shapes of the plans there are so far; None where no pages are shared to any use."""
         if self.meta.shared is None:
             return None
-        return tuple((key, plan.shape if pays(self.meta) else None) for key, (plan, pays) in self.shared_plans.items())
+        return (self.worth(self.meta) if self.worth is not None else (),
+                *((key, plan.shape if pays(self.meta) else None) for key, (plan, pays) in self.shared_plans.items()))
 
     def _range_place(self, i):
         first = 7 * self.batch_size + 1 + i * (self.batch_size + 2)
@@ -290,7 +293,7 @@ class StaticDecodeMeta:
         m.num_real = n
         m.shared = None if shared is None else shared.filled_up(B)
         if shared is not None:
-            if self.shared_plans and not any(pays(m) for _, pays in self.shared_plans.values()):
+            if self.worth is not None and not any(self.worth(m)):
                 m.shared = None
             for plan, pays in self.shared_plans.values():
                 if m.shared is not None and pays(m):

@@ -17,6 +17,7 @@ import torch
 from ..cache import PAGE_TOKENS, Cache, pages_for
 from ..config import load_config
 from ..errors import BackendError, ModelLoadError, NeedsEagerStep, RequestError
+from ..kernels.shared import worth_over
 from ..parts import Runtime
 from ..weights import read_tensor, read_tensors
 
@@ -85,11 +86,12 @@ class Engine:
         self.static_decode = self.model.graph_safe
         self.use_graphs = bool(use_graphs) and self.model.graph_safe
         self._decode = OrderedDict()    # batch size -> _DecodeState, least recently used first
-        self._graphs = OrderedDict()    # (batch size, context bucket, unequal, shared plan's shape) -> graph, least recently used first
+        self._graphs = OrderedDict()    # (batch size, context bucket, unequal, StaticDecodeMeta.shared_shape) -> graph, least recently used first
         self._shared_logits = None      # [rows, vocab], made by the first decode step, grown by a larger batch
         self._capture_stream = None     # the stream that graphs are captured on
         self._sized_rows = 0            # the largest decode step that has run outside a graph: buffers for it exist
         self.graphs_captured = 0
+        self._worth = worth_over(self.cache.kv_groups, self.rt.dtype)
         self._sharing = (None, None)    # (the cache's version of what is shared, slots) of a step, its SharedPages
         self.ignored_tensors = []       # stored tensors that the model did not ask for
         self._tensor_source = None      # how get_tensor finds a tensor again: set by the constructors below
@@ -281,7 +283,7 @@ class Engine:
         whose sequences end one after another then meets few new shapes instead of one a sequence.
         A graph is tied to that batch size, to the bucket of the longest context (which sizes the
         attention grid), to whether the contexts are of very unequal lengths (the attention then
-        deals its grid out by a list) and, where sequences share pages, to the size of that plan. All graphs write their logits into the first rows of the
+        deals its grid out by a list) and, where sequences share pages, to whether reading them together pays and the size of that plan. All graphs write their logits into the first rows of the
         engine's one buffer; what is returned here is a view of those rows, which the next decode
         step writes again (`step` copies it for callers that keep it). At most MAX_GRAPHS graphs and
         MAX_DECODE_BATCH_SIZES batch sizes are kept, the least recently used go first. `set_aside` is called before
@@ -304,7 +306,7 @@ class Engine:
                 self._shared_logits = None
                 self._shared_logits = torch.empty((rows, self.spec.vocab_size), dtype=torch.float32,
                                                   device=self.device)
-            state = self._decode[B] = _DecodeState(StaticDecodeMeta(B, self.device, self.cache.pad_slot),
+            state = self._decode[B] = _DecodeState(StaticDecodeMeta(B, self.device, self.cache.pad_slot, self._worth),
                                                    self._shared_logits[:B])
         self._decode.move_to_end(B)
         meta = state.static.update(entries, starts, shared)

@@ -223,6 +223,13 @@ def _ends_sooner(meta, nkv, hd, dtype):
     return _saved(meta, nkv, hd, dtype) >= SAVED_BYTES + SAVED_BYTES_EACH * min(meta.num_seqs, SAVED_SEQUENCES)
 
 
+def worth_over(needs, dtype):
+    """A function of a step's BatchMeta: of each kind of cache among `needs` (KVNeeds) whose pages may be read together, whether that pays.
+    A recorded step is tied to its answers: they are known before any layer has asked for a plan."""
+    kinds = sorted({(n.kv_heads, n.head_dim) for n in needs if n.values and not n.window})
+    return lambda meta: tuple(_ends_sooner(meta, nkv, hd, dtype) for nkv, hd in kinds)
+
+
 def _plan_of(meta, nq, nkv, hd, dtype):
     key = ("shared_plan", nq // nkv, nkv, hd, dtype)
     if meta.static is not None:

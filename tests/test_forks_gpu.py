@@ -12,7 +12,7 @@ from herbert_rs_amd.errors import CacheError, RequestError
 from herbert_rs_amd.kernels import shared
 
 from .bounds import BF16_REL_RMS, F32_ABS, close
-from .plain_cache import plain_logits
+from .plain_cache import forget, plain_logits, plain_rows
 from .tiny import CONFIGS, make_folder, random_tokens
 
 pytestmark = pytest.mark.gpu
@@ -357,3 +357,49 @@ def test_the_command_line_prints_samples_and_log_probabilities(model_root, capsy
     assert main(args + ["--logprobs", "0"]) == 0
     assert sum("\t" in l for l in capsys.readouterr().out.splitlines()) == 5
     assert main(args + ["--samples", "0"]) == 1
+
+
+def test_a_step_that_comes_to_pay_is_not_replayed_as_it_was(model_root, monkeypatch):
+    """With the thresholds as they are: steps of 24 sequences of which two share pages, recorded without the shared attention, then the same
+    size and length with all of them behind one prompt, then the first again."""
+    calls, real = [], shared.attention
+    monkeypatch.setattr(shared, "attention", lambda *args, **kw: calls.append(args[0].shape[0]) or real(*args, **kw))
+    folder, vocab = make_folder(model_root, "F", "bfloat16", {"head_dim": 128}), CONFIGS["F"][0]["vocab_size"]
+    engine = hb.load(folder, dtype="bfloat16", cache_tokens=64 * 24 * 32, max_slots=24)
+    texts = {}
+
+    def begin(prompts, forks):
+        for slot in list(texts):
+            engine.free_slot(slot)
+            del texts[slot]
+        for p in prompts:
+            slot = engine.alloc_slot()
+            engine.step([StepEntry(slot, p, [])])
+            texts[slot] = list(p)
+        for new in engine.fork(slot, forks):
+            texts[new] = list(p)
+
+    def go_on(steps, seed):
+        calls.clear()
+        for at in range(steps):
+            for s in texts:
+                texts[s] = texts[s] + random_tokens(vocab, 1, 100 * seed + 10 * at + s)
+            rows = engine.step([StepEntry(s, t[-1:], [0]) for s, t in texts.items()]).cpu().numpy()
+        for s in (min(texts), max(texts)):
+            row = rows[list(texts).index(s)]
+            ok, err = close(row, plain_rows(folder, texts[s], [len(texts[s]) - 1])[len(texts[s]) - 1], "bfloat16", "F", "coming to pay")
+            assert ok, f"slot {s}: {err}"
+        return list(calls)
+    apart = [random_tokens(vocab, 1800, 50 + i) for i in range(23)]
+    begin(apart, 1)
+    assert go_on(4, 1) == []
+    recorded = engine.graphs_captured
+    assert recorded >= 1
+    begin([random_tokens(vocab, 1800, 90)], 23)
+    assert go_on(4, 2) and all(n == 24 for n in calls)
+    assert engine.graphs_captured > recorded
+    recorded = engine.graphs_captured
+    begin(apart, 1)
+    assert go_on(2, 3) == [] and engine.graphs_captured == recorded
+    engine.cache.check()
+    forget(folder)

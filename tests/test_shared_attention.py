@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 import torch
 
-from herbert_rs_amd.cache import LayerKV, shared_pages
+from herbert_rs_amd.cache import KVNeed, LayerKV, shared_pages
 from herbert_rs_amd.cache.sharing import MAX_LEVELS
 from herbert_rs_amd.engine import StepEntry, batch
 from herbert_rs_amd.errors import BackendError
@@ -168,3 +168,30 @@ def call(**changed):
 def test_calls_that_the_entry_refuses(changed, text):
     with pytest.raises(BackendError, match=text):
         call(**changed)
+
+
+def decoding(pages, shared_by, count, static, held=None):
+    """A decode step of `count` sequences of which the first `shared_by` hold the same `pages` pages, and `static` after it."""
+    table, _ = tables([[("p", pages), (None, 1)] if i < shared_by else [(None, pages + 1)] for i in range(count)], 3)
+    held = held or [64 * pages + 5] * count
+    return static.update([StepEntry(i, [1], [0]) for i in range(count)], held, shared_pages(table, held))
+
+
+def test_what_a_recorded_step_is_tied_to_says_whether_sharing_pays():
+    """Known before any plan is made: a step that was recorded where nothing is gained is not replayed where something is."""
+    needs = [KVNeed(8, 128), KVNeed(8, 128, 256), KVNeed(1, 32), KVNeed(4, 128, values=False)]
+    static = batch.StaticDecodeMeta(64, "cpu", 99, shared.worth_over(needs, torch.bfloat16))
+    decoding(100, 2, 64, static)
+    few = static.shared_shape, static.meta.context_bucket, static.meta.unequal
+    assert static.meta.shared is None and few[0] is None
+    decoding(100, 64, 64, static)
+    assert static.meta.shared is not None and (static.shared_shape, static.meta.context_bucket, static.meta.unequal) != few
+    assert static.shared_shape == ((False, True),)                 # (a head of 32: 52 MB saved of 152)
+    decoding(900, 64, 64, static)
+    assert static.shared_shape == ((True, True),)
+    decoding(100, 2, 64, static)
+    assert static.shared_shape is None
+    # a plan that one kind of heads has made, and does not pay for now, does not keep the other kind from theirs
+    static.shared_plans["small heads"] = (None, lambda m: False)
+    decoding(100, 64, 64, static)
+    assert static.meta.shared is not None and static.shared_shape == ((False, True), ("small heads", None))
