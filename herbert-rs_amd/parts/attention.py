@@ -36,7 +36,7 @@ head are two query heads of one kept key, which holds both maps' keys side by si
 the other map lies: the values are kept and read once.
 
 Where sequences of a step share pages (forked slots), either form without window, chunks and biases by distance reads
-those pages once for all of them where that ends sooner (kernels.shared), one map a head.
+those pages once for all of them where that ends sooner (kernels.shared), one map a head (in float32 also two).
 
 Three further options go with either form (not in the reference): `keep_first` (with a window: the sequence's first
 so many keys are seen as well; the cache keeps their pages), `distance_bias=(bias_max,)` (a learned bias by the
@@ -316,7 +316,7 @@ class Attention(Part):
         angles, rot_dims, halves = self.position.step_angles(ctx) if hasattr(self.position, "step_angles") else (None, 0, False)
         gate_off = L.channels if self.gate else None
         plain_masks = not self.keep_first and self.distance_raw is None
-        shares = self.maps == 1 and self._shares(ctx, kv)
+        shares = self._shares(ctx, kv)
         fused = plain_masks and not shares and mfma.decode_heads_fusable(meta, kv, L, rt.dtype)
         cores = plain_masks and not shares and mfma.heads_supported(kv, L, rt.dtype)
         # (slices of K are added up by the kernels that read the projection, but for the one that only gates heads)
@@ -479,9 +479,10 @@ class Attention(Part):
         self.project_out(ctx, attn, x)
 
     def _shares(self, ctx, kv):
-        """True where pages that several sequences of the step hold are read once for all of them."""
+        """True where pages that several sequences of the step hold are read once for all of them. (Two maps a head: in float32 alone, where
+        their difference is taken after the attention; in bfloat16 the kernel that attends takes it.)"""
         return (ctx.meta.shared is not None and not self.window and self.chunk is None and self.distance_raw is None
-                and shared.pays(ctx.meta, kv, self.kept_heads, self.nkv, self.hd, ctx.rt.dtype))
+                and (self.maps == 1 or ctx.rt.dtype == torch.float32) and shared.pays(ctx.meta, kv, self.kept_heads, self.nkv, self.hd, ctx.rt.dtype))
 
     def attend(self, ctx, q, kv, out):
         scale = self.scale if self.prepared else self.kernel_scale

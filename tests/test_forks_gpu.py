@@ -403,3 +403,29 @@ def test_a_step_that_comes_to_pay_is_not_replayed_as_it_was(model_root, monkeypa
     assert go_on(2, 3) == [] and engine.graphs_captured == recorded
     engine.cache.check()
     forget(folder)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_forks_through_heads_of_two_maps(dtype, used, model_root, monkeypatch):
+    """Two maps a head: shared pages are read together as for twice the heads in float32, and by the layers' own kernel in bfloat16."""
+    from . import figalorn_tiny
+    counted, heads = shared.attention, []
+    monkeypatch.setattr(shared, "attention", lambda *args, **kw: heads.append(args[4]) or counted(*args, **kw))
+    folder, vocab = figalorn_tiny.make_folder(model_root, "R", dtype), figalorn_tiny.CONFIGS["R"][0]["vocab"]
+    engine = hb.load(folder, dtype=dtype, cache_tokens=64 * 30, max_slots=8)
+    prompt, ways = random_tokens(vocab, 140, 1), [random_tokens(vocab, 10, 30 + i) for i in range(4)]
+    got = []
+    for forked in (True, False):
+        first = engine.alloc_slot()
+        engine.step([StepEntry(first, prompt, [])])
+        slots = [first] + (engine.fork(first, 3) if forked else [engine.alloc_slot() for _ in range(3)])
+        for s in slots[1:] if not forked else ():
+            engine.step([StepEntry(s, prompt, [])])
+        got.append([engine.step([StepEntry(s, [w[at]], [0]) for s, w in zip(slots, ways)]).cpu() for at in range(10)])
+        for s in slots:
+            engine.free_slot(s)
+    assert set(heads) == ({1, 2} if dtype == "float32" else {1})        # (a layer of one head, and one of one head with two maps)
+    if dtype == "float32":                                              # (sums in another order; bfloat16: see the test of every family)
+        for a, b in zip(*got):
+            assert (a - b).abs().max() <= F32_ABS
+    engine.cache.check()

@@ -1,15 +1,19 @@
 """Which pages sequences share, how a step is cut into items, and what the shared attention refuses (no GPU needed)."""
+from types import SimpleNamespace
+
 import numpy as np
 import pytest
 import torch
 
-from herbert_rs_amd.cache import KVNeed, LayerKV, shared_pages
+from herbert_rs_amd.cache import KVNeed, LayerKV, SharedPages, shared_pages
 from herbert_rs_amd.cache.sharing import MAX_LEVELS
-from herbert_rs_amd.engine import StepEntry, batch
+from herbert_rs_amd.engine import Model, StepEntry, batch
 from herbert_rs_amd.errors import BackendError
 from herbert_rs_amd.kernels import lib, shared
 
+from . import figalorn_tiny
 from .shared_util import tables
+from .tiny import spec_of
 
 
 def as_sets(found, table, held):
@@ -195,3 +199,17 @@ def test_what_a_recorded_step_is_tied_to_says_whether_sharing_pays():
     static.shared_plans["small heads"] = (None, lambda m: False)
     decoding(100, 64, 64, static)
     assert static.meta.shared is not None and static.shared_shape == ((False, True), ("small heads", None))
+
+
+@pytest.mark.parametrize("dtype, taken", [(torch.float32, True), (torch.bfloat16, False)])
+def test_heads_of_two_maps_share_in_float32_alone(dtype, taken):
+    """In bfloat16 the kernel that attends takes the maps from each other as well: what a layer says of itself is what it does."""
+    mixer = Model(spec_of(figalorn_tiny.CONFIGS["F"][0])[1]).blocks[0].mixer
+    assert mixer.maps == 2 and mixer.chunk is None and mixer.window is None
+    nodes = [(0, 64, 0, 1000)] + [(i, 1, 1000, -1) for i in range(64)]
+    meta = SimpleNamespace(shared=SharedPages(np.arange(64), nodes), max_new=1, num_seqs=64, num_tokens=64)
+    kv = LayerKV(torch.zeros(1, mixer.nkv, 64, mixer.hd, dtype=dtype), torch.zeros(1, mixer.nkv, mixer.hd, 64, dtype=dtype),
+                 torch.zeros(1, 1, dtype=torch.int32), 64, 0)
+    ctx = SimpleNamespace(meta=meta, rt=SimpleNamespace(dtype=dtype))
+    assert shared.pays(meta, kv, mixer.kept_heads, mixer.nkv, mixer.hd, dtype)
+    assert mixer._shares(ctx, kv) == taken
