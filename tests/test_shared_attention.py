@@ -213,3 +213,37 @@ def test_heads_of_two_maps_share_in_float32_alone(dtype, taken):
     ctx = SimpleNamespace(meta=meta, rt=SimpleNamespace(dtype=dtype))
     assert shared.pays(meta, kv, mixer.kept_heads, mixer.nkv, mixer.hd, dtype)
     assert mixer._shares(ctx, kv) == taken
+
+
+def decode_of(count, shared_places, context, shared_by=None):
+    """What `pays` looks at, of a decode step of `count` sequences (the first `shared_by` of which share so many pages)."""
+    shared_by = shared_by or count
+    nodes = [(0, shared_by, 0, shared_places)] + [(i, 1, shared_places if i < shared_by else 0, -1) for i in range(count)]
+    return SimpleNamespace(shared=SharedPages(np.arange(count), nodes), max_new=1, num_seqs=count, num_tokens=count,
+                           host_context=np.full(count, context))
+
+
+def cache_of(nkv, hd, dtype):
+    return LayerKV(torch.zeros(1, nkv, 64, hd, dtype=dtype), torch.zeros(1, nkv, hd, 64, dtype=dtype), torch.zeros(1, 1, dtype=torch.int32), 64, 0)
+
+
+@pytest.mark.parametrize("count, pages, taken", [
+    # 8 kv heads of 128: a page that one sequence more does not read is 256 KiB; 32 MiB and 6 MiB a sequence are asked for
+    (2, 175, False), (2, 176, True), (8, 45, False), (8, 46, True), (20, 31, False), (20, 32, True),
+    # ... of 20 sequences at most
+    (64, 9, False), (64, 10, True), (128, 4, False), (128, 5, True)])
+def test_how_much_has_to_be_saved(count, pages, taken):
+    assert shared.pays(decode_of(count, pages, 64 * pages + 9), cache_of(8, 128, torch.bfloat16), 32, 8, 128, torch.bfloat16) == taken
+    # (in float32 whatever is shared is worth it)
+    assert shared.pays(decode_of(count, 1, 100), cache_of(8, 128, torch.float32), 32, 8, 128, torch.float32)
+
+
+@pytest.mark.parametrize("dtype, most", [(torch.bfloat16, 8), (torch.float32, 200)])
+def test_steps_of_many_tokens_a_sequence_are_prompts(dtype, most):
+    kv = cache_of(8, 128, dtype)
+    for tokens, taken in ((24 * most, True), (24 * most + 1, False)):
+        meta = decode_of(24, 1000, 64 * 1000 + most + 50)
+        meta.max_new, meta.num_tokens = most + 50, tokens
+        assert shared.pays(meta, kv, 32, 8, 128, dtype) == taken
+    meta.max_new, meta.shared = 1, None
+    assert not shared.pays(meta, kv, 32, 8, 128, dtype)
