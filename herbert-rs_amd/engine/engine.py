@@ -91,7 +91,7 @@ class Engine:
         self._capture_stream = None     # the stream that graphs are captured on
         self._sized_rows = 0            # the largest decode step that has run outside a graph: buffers for it exist
         self.graphs_captured = 0
-        self._worth = worth_over(self.cache.kv_groups, self.rt.dtype)
+        self._worth = worth_over(self.cache.kv_groups, self.rt.dtype, self.model.heads_prepared_alone())
         self._sharing = (None, None)    # (the cache's version of what is shared, slots) of a step, its SharedPages
         self.ignored_tensors = []       # stored tensors that the model did not ask for
         self._tensor_source = None      # how get_tensor finds a tensor again: set by the constructors below

@@ -107,6 +107,9 @@ class Model:
                     needs[i] = need
         return needs
 
+    def heads_prepared_alone(self):
+        return {h for b in self.blocks for h in getattr(getattr(b, "mixer", None), "heads_prepared_alone", tuple)()}
+
     # ---- one step
     def forward(self, rt, meta, cache, logits_out=None):
         """float32 logits [wanted rows, vocab] (None when nothing is wanted); written into

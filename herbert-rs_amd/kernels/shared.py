@@ -41,6 +41,16 @@ BY_ITSELF_PAGES = 6
 SAVED_BYTES = 32 << 20
 SAVED_BYTES_EACH = 6 << 20      # and these for each sequence, of SAVED_SEQUENCES at most
 SAVED_SEQUENCES = 20
+# Where a kernel of its own norms, rotates and writes in any case (a filter along time, a cache that another entry fills, part of a head rotated), a step
+# whose sequences are items of their own ends sooner than by the attention of one sequence after another at heads of up to so many entries, so
+# many sequences x kv heads, and from the page behind so many on. A model's decode steps, microseconds that whole rows save of 710 to 900, 12 filtered
+# layers, prompts of 70, 134, 198 and 326 tokens: 16 heads of 64 over 4, 2 sequences 5, 1, 6, 10, 8 sequences 9, 3, 8, 18, 16 sequences 5, 2, 8, 18, 32 sequences
+# 0, -1, 1, 0; over 16, 2 sequences 1, -1, 4, 11, 8 sequences 6, 1, 6, -2; 16 heads of 32 over 2, 2 sequences 2, 0, 4, 20, 8 sequences 4, 4, 10, 28, 16 sequences 0,
+# 3, 5, 24; 8 over 8, 2 sequences 0, -5, 1, 18, 8 sequences -5, -6, 0, 18. Heads of 128 by themselves: 2 sequences of 4 kv heads 5.6, 6.4, 7.7, 7.1 us separate,
+# 6.0, 6.9, 7.7, 9.0 as whole rows.
+ALONE_DIM = 64
+ALONE_PAIRS = 64
+ALONE_PAGES = 3
 # Tokens a sequence from which a step is worth more as a prompt: its own columns fill the products by then. 24 sequences of 8, 40 and 200 new tokens behind
 # 2,000 shared ones: 28, 46, 157 us shared, 34, 38, 121 us separate; behind 1,000: 23, 40, 128 and 23, 27, 80 us. In float32 16 sequences of 8, 40 and
 # 200 behind 256: 15, 38, 135 us shared, 21, 33, 129 us separate; behind 2,000: 37, 128, 526 and 98, 146, 566 us.
@@ -207,34 +217,39 @@ def _saved(meta, nkv, hd, dtype):
     return meta.shared.pages_saved * nkv * 64 * hd * 2 * (4 if dtype == torch.float32 else 2)
 
 
-def pays(meta, kv, nq, nkv, hd, dtype):
+def pays(meta, kv, nq, nkv, hd, dtype, alone=False):
     """True where the shared attention takes this step over this cache and ends sooner than the attention that reads every sequence's pages
-    by itself: by the bytes of keys and values that are not read again."""
-    return meta.shared is not None and supported(kv, nq, nkv, hd, dtype) and _ends_sooner(meta, nkv, hd, dtype)
+    by itself: by the bytes of keys and values that are not read again, or, where queries, keys and values are prepared by a kernel of their own
+    in any case (alone), in steps of four to six pages."""
+    return meta.shared is not None and supported(kv, nq, nkv, hd, dtype) and _ends_sooner(meta, nkv, hd, dtype, alone)
 
 
-def _ends_sooner(meta, nkv, hd, dtype):
+def _ends_sooner(meta, nkv, hd, dtype, alone=False):
     if meta.shared is None:
         return False
     if meta.max_new > 1 and meta.num_tokens > MANY_TOKENS[dtype] * meta.num_seqs:
         return False
     if dtype == torch.float32:          # (8 sequences of 128 tokens: 11 us shared, 17 separate; of 2,048: 17 and 103)
         return True
+    if alone and hd <= ALONE_DIM and meta.num_seqs * nkv <= ALONE_PAIRS and _by_itself(meta, nkv, dtype):
+        return int(meta.host_context.max()) > 64 * ALONE_PAGES
     return _saved(meta, nkv, hd, dtype) >= SAVED_BYTES + SAVED_BYTES_EACH * min(meta.num_seqs, SAVED_SEQUENCES)
 
 
-def worth_over(needs, dtype):
+def worth_over(needs, dtype, alone=()):
     """A function of a step's BatchMeta: of each kind of cache among `needs` (KVNeeds) whose pages may be read together, whether that pays.
-    A recorded step is tied to its answers: they are known before any layer has asked for a plan."""
+    alone: (kv heads, head size) of those that are read where a kernel of its own prepares (see pays). A recorded step is tied to its
+    answers: they are known before any layer has asked for a plan."""
     kinds = sorted({(n.kv_heads, n.head_dim) for n in needs if n.values and not n.window})
-    return lambda meta: tuple(_ends_sooner(meta, nkv, hd, dtype) for nkv, hd in kinds)
+    kinds = [(*k, False) for k in kinds] + [(*k, True) for k in kinds if k in set(alone)]
+    return lambda meta: tuple(_ends_sooner(meta, nkv, hd, dtype, by_itself) for nkv, hd, by_itself in kinds)
 
 
-def _plan_of(meta, nq, nkv, hd, dtype):
-    key = ("shared_plan", nq // nkv, nkv, hd, dtype)
+def _plan_of(meta, nq, nkv, hd, dtype, alone):
+    key = ("shared_plan", nq // nkv, nkv, hd, dtype, alone)
     if meta.static is not None:
         found = meta.static.shared_plan(key, lambda rows, device: StaticPlan(nq // nkv, nkv, dtype, rows, device),
-                                        lambda m: _ends_sooner(m, nkv, hd, dtype))
+                                        lambda m: _ends_sooner(m, nkv, hd, dtype, alone))
         if found is None:
             raise BackendError("shared attention: it does not pay for this step (see pays)")
         return found
@@ -245,12 +260,12 @@ def _plan_of(meta, nq, nkv, hd, dtype):
     return found
 
 
-def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, scratch=None):
+def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, scratch=None, alone=False):
     """Causal attention of the step's tokens over their slots' pages, a page that several sequences share read once for all of
     them. q, out [T, nq hd] in the cache's dtype, bfloat16 (heads of 32, 64 or 128) or float32 (up to 256, a multiple of 4); meta.shared: a cache.SharedPages of
     the step's sequences. sinks f32 [nq]: the softmax's denominator of head h also holds exp(sinks[h]). softcap: a scaled score s
     becomes softcap tanh(s / softcap). scratch: a mfma.Scratch whose memory the partial results take, for one call (or recorded graph) at a
-    time; None: memory of this call's own. meta is used on the stream that it was packed on."""
+    time; None: memory of this call's own. alone: as it was told `pays`. meta is used on the stream that it was packed on."""
     T = q.shape[0]
     if meta.shared is None:
         raise BackendError("shared attention: the sequences of this step share no pages")
@@ -264,7 +279,7 @@ def attention(q, meta, kv, out, nq, nkv, hd, scale, sinks=None, softcap=None, sc
                    meta.slots, i32, (meta.num_seqs,), *further)
     if meta.max_context > 64 * table.shape[1]:
         raise BackendError(f"shared attention: a context of {meta.max_context} tokens does not fit a table of {table.shape[1]} pages")
-    p = _plan_of(meta, nq, nkv, hd, q.dtype)
+    p = _plan_of(meta, nq, nkv, hd, q.dtype, alone)
     if p.direct:
         po = pml = None
     elif scratch is None:

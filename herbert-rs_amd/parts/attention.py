@@ -482,13 +482,25 @@ class Attention(Part):
         """True where pages that several sequences of the step hold are read once for all of them. (Two maps a head: in float32 alone, where
         their difference is taken after the attention; in bfloat16 the kernel that attends takes it.)"""
         return (ctx.meta.shared is not None and not self.window and self.chunk is None and self.distance_raw is None
-                and (self.maps == 1 or ctx.rt.dtype == torch.float32) and shared.pays(ctx.meta, kv, self.kept_heads, self.nkv, self.hd, ctx.rt.dtype))
+                and (self.maps == 1 or ctx.rt.dtype == torch.float32)
+                and shared.pays(ctx.meta, kv, self.kept_heads, self.nkv, self.hd, ctx.rt.dtype, self.prepares_alone))
+
+    @property
+    def prepares_alone(self):
+        """True where a kernel of its own prepares queries, keys and values of single tokens as well, which the decode attention else does."""
+        if self.filtered or self.reads_cache_only:
+            return True
+        rotation = None if self.prepared else self.position.rotation()
+        return rotation is not None and rotation[2] not in (0, self.hd)
+
+    def heads_prepared_alone(self):
+        return ((self.nkv, self.hd),) if self.prepares_alone else ()
 
     def attend(self, ctx, q, kv, out):
         scale = self.scale if self.prepared else self.kernel_scale
         if out.dtype == q.dtype and self._shares(ctx, kv):
             shared.attention(q, ctx.meta, kv, out, self.kept_heads, self.nkv, self.hd, scale, sinks=self.sink_w, softcap=self.softcap,
-                             scratch=ctx.rt.scratch)
+                             scratch=ctx.rt.scratch, alone=self.prepares_alone)
             return
         if q.dtype == torch.bfloat16:
             if out.dtype == q.dtype and mfma.attention_supported(q, kv, self.kept_heads, self.nkv, self.hd):

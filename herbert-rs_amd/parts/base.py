@@ -49,6 +49,10 @@ class Part:
     def cache_need(self):
         return None
 
+    def heads_prepared_alone(self):
+        """(kv heads, head size) of a mixer's attentions that are always preceded by a kernel of their own (see kernels.shared.pays)."""
+        return ()
+
 
 class Runtime:
     """Compute dtype, device and the scratch buffers that all layers share."""

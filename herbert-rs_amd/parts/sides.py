@@ -63,6 +63,9 @@ class SideBySide(Part):
         needs = tuple(n for m in self.sides for n in _needs_of(m))
         return needs or None
 
+    def heads_prepared_alone(self):
+        return tuple(h for m in self.sides for h in m.heads_prepared_alone())
+
     def load(self, tensors, rt):
         for m in self.sides:
             m.load(tensors, rt)

@@ -247,3 +247,27 @@ def test_steps_of_many_tokens_a_sequence_are_prompts(dtype, most):
         assert shared.pays(meta, kv, 32, 8, 128, dtype) == taken
     meta.max_new, meta.shared = 1, None
     assert not shared.pays(meta, kv, 32, 8, 128, dtype)
+
+
+@pytest.mark.parametrize("count, context, nkv, hd, taken", [
+    (2, 192, 4, 64, False), (2, 193, 4, 64, True), (16, 384, 4, 64, True), (16, 385, 4, 64, False), (17, 200, 4, 64, False), (4, 200, 16, 64, True),
+    (5, 200, 16, 64, False), (2, 200, 4, 128, False), (2, 200, 2, 32, True)])
+def test_short_contexts_behind_a_kernel_of_their_own_are_read_sequence_by_sequence(count, context, nkv, hd, taken):
+    """The steps whose sequences are items of their own, as a filtered attention's decode step takes them; and the attention that prepares
+    its rows itself does not."""
+    meta, kv = decode_of(count, 1, context), cache_of(nkv, hd, torch.bfloat16)
+    assert shared.pays(meta, kv, 4 * nkv, nkv, hd, torch.bfloat16, True) == taken
+    assert not shared.pays(meta, kv, 4 * nkv, nkv, hd, torch.bfloat16)
+    assert shared.worth_over([KVNeed(nkv, hd)], torch.bfloat16, {(nkv, hd)})(meta) == (False, taken)
+    assert shared.worth_over([KVNeed(nkv, hd)], torch.bfloat16)(meta) == (False,)
+    if taken:
+        meta.host_starts, meta.host_slots = np.arange(count + 1), np.arange(count)
+        items, order, part_start, parts, most, direct = shared._planned(meta, 4, nkv, torch.bfloat16)
+        assert direct and len(items) == count and most == 1
+
+
+def test_which_layers_prepare_by_a_kernel_of_their_own():
+    from . import mefatar_tiny, vipalorn_tiny
+    assert Model(spec_of(mefatar_tiny.CONFIGS["Q"][0])[1]).heads_prepared_alone() == {(4, 64), (2, 64)}
+    assert Model(spec_of(figalorn_tiny.CONFIGS["F"][0])[1]).heads_prepared_alone() == set()
+    assert Model(spec_of(vipalorn_tiny.CONFIGS["Q"][0])[1]).heads_prepared_alone() == set()
