@@ -480,8 +480,9 @@ class Attention(Part):
 
     def _shares(self, ctx, kv):
         """True where pages that several sequences of the step hold are read once for all of them. (Two maps a head: in float32 alone, where
-        their difference is taken after the attention; in bfloat16 the kernel that attends takes it.)"""
-        return (ctx.meta.shared is not None and not self.window and self.chunk is None and self.distance_raw is None
+        their difference is taken after the attention; in bfloat16 the kernel that attends takes it. A scale that is not positive goes
+        with the ordinary attention of float32 alone.)"""
+        return (ctx.meta.shared is not None and not self.window and self.chunk is None and self.distance_raw is None and self.scale > 0
                 and (self.maps == 1 or ctx.rt.dtype == torch.float32)
                 and shared.pays(ctx.meta, kv, self.kept_heads, self.nkv, self.hd, ctx.rt.dtype, self.prepares_alone))
 

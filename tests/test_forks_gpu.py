@@ -1,5 +1,6 @@
 """Forked slots, several answers to a prompt, log probabilities and scoring through the engine."""
 import importlib
+import json
 import math
 
 import numpy as np
@@ -463,3 +464,21 @@ def test_forks_behind_a_filter_pass_from_short_contexts_to_longer_ones(graphs, m
     for s in slots:
         engine.free_slot(s)
     engine.cache.check()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_forks_of_a_model_whose_scores_have_a_scale_that_is_not_positive(scale, used, tmp_path):
+    from . import mefatar_tiny
+    raw = json.loads(json.dumps(mefatar_tiny.CONFIGS["Q"][0]))
+    for layer in (1, 3):
+        raw["layers"][layer]["mixer"]["left"]["scale"] = scale
+    hb.write_random_model(str(tmp_path), raw, seed=5, dtype="float32", std=0.09, norm_std=0.1)
+    engine = hb.load(str(tmp_path), dtype="float32", cache_tokens=64 * 12)
+    prompt, ways = random_tokens(raw["vocab"], 75, 1), [random_tokens(raw["vocab"], 6, 30 + i) for i in range(3)]
+    first = engine.alloc_slot()
+    engine.step([StepEntry(first, prompt, [])])
+    slots = [first] + engine.fork(first, 2)
+    rows = [engine.step([StepEntry(s, [w[at]], [0]) for s, w in zip(slots, ways)]).cpu().numpy() for at in range(6)]
+    for i, w in enumerate(ways):
+        ref = mefatar_tiny.plain_logits(str(tmp_path), prompt + w)
+        assert all(close(rows[at][i], ref[75 + at], "float32", "mef", "turned scores")[0] for at in range(6))

@@ -1,4 +1,5 @@
 """Which pages sequences share, how a step is cut into items, and what the shared attention refuses (no GPU needed)."""
+import json
 from types import SimpleNamespace
 
 import numpy as np
@@ -271,3 +272,14 @@ def test_which_layers_prepare_by_a_kernel_of_their_own():
     assert Model(spec_of(mefatar_tiny.CONFIGS["Q"][0])[1]).heads_prepared_alone() == {(4, 64), (2, 64)}
     assert Model(spec_of(figalorn_tiny.CONFIGS["F"][0])[1]).heads_prepared_alone() == set()
     assert Model(spec_of(vipalorn_tiny.CONFIGS["Q"][0])[1]).heads_prepared_alone() == set()
+
+
+@pytest.mark.parametrize("scale, taken", [(0.125, True), (0.0, False), (-0.125, False)])
+def test_scores_with_a_scale_that_is_not_positive_stay_with_the_ordinary_attention(scale, taken):
+    """In float32 that one takes any scale, and a configuration may name one."""
+    from . import mefatar_tiny
+    raw = json.loads(json.dumps(mefatar_tiny.CONFIGS["Q"][0]))
+    raw["layers"][1]["mixer"]["left"]["scale"] = scale
+    mixer = Model(spec_of(raw)[1]).blocks[1].mixer.sides[0]
+    ctx = SimpleNamespace(meta=decode_of(4, 2, 130), rt=SimpleNamespace(dtype=torch.float32))
+    assert mixer._shares(ctx, cache_of(mixer.nkv, mixer.hd, torch.float32)) == taken
