@@ -8,6 +8,7 @@ import os
 from .config import load_config, read_config_json
 from .config.registry import resolve_architecture
 from .engine import Engine
+from .engine.engine import SCORED_ROWS
 from .engine.model import Model
 from .sampling import SamplingParams
 from .weights import write_model_folder
@@ -35,8 +36,11 @@ def generate(model, prompts, temperature=0.4, top_k=40, top_p=0.9, max_tokens=20
     if isinstance(model, Engine):
         engine = model
     else:
-        further = (samples - 1) * ((max_tokens + 190) // 64 * 64)       # (what another answer holds beside the prompt's whole pages)
-        room = sum((len(p) + max_tokens + 127) // 64 * 64 + further for p in plist[:max_batch])
+        params.validate()
+        # what runs at once: so many prompts at most, and the other answers, each with what it holds beside its prompt's whole pages
+        at_once = plist[:max_batch] if samples == 1 else sorted(plist, key=len)[-((max_batch - 2) // samples + 2):]
+        further = min(len(at_once) * (samples - 1), max_batch - 1) * ((max_tokens + 190) // 64 * 64)
+        room = sum((len(p) + max_tokens + 127) // 64 * 64 for p in at_once) + further
         engine = load(model, dtype=dtype, cache_tokens=room)
     results = engine.generate(plist, params, max_batch=max_batch, prefill_chunk=prefill_chunk)
     tokens = [r.tokens for r in results]
@@ -49,7 +53,7 @@ def score(model, prompt, continuations, top=0, dtype="bfloat16"):
     """What a model (a folder or an Engine) says of given continuations of a prompt, all as token ids: for each a list of
     sampling.logprobs.TokenLogprob. See Engine.score."""
     if not isinstance(model, Engine):
-        room = len(prompt) + 128 + sum((len(c) + 191) // 64 * 64 for c in continuations)
+        room = len(prompt) + 128 + sum((n + 191) // 64 * 64 for n in sorted(map(len, continuations))[-SCORED_ROWS:])
         model = load(model, dtype=dtype, cache_tokens=room)
     return model.score(prompt, continuations, top)
 

@@ -247,6 +247,7 @@ def main(argv=None):
 
 def _run(args):
     from .api import load, write_random_model
+    from .engine.engine import MAX_BATCH
     from .sampling import INTERRUPTED, SamplingParams
     if args.arch:
         return print_arch()
@@ -327,7 +328,8 @@ def _run(args):
     samples = args.samples
     if samples < 1:
         raise RequestError("--samples must be at least 1")
-    cache_tokens = args.cache_tokens or (len(ids) + args.max_tokens + 65 + (samples - 1) * (args.max_tokens + 192))
+    further = min(samples, MAX_BATCH) - 1           # (answers beside the first that run at once)
+    cache_tokens = args.cache_tokens or (len(ids) + args.max_tokens + 65 + further * (args.max_tokens + 192))
     engine = load(args.model, dtype=args.dtype, cache_tokens=cache_tokens)
     load_seconds = time.perf_counter() - t0
 

@@ -54,6 +54,8 @@ MAX_GRAPHS = 192
 SHARED_LOGITS_ROWS = 64
 # Rows of logits that scoring asks for in one step (311 MB for a vocabulary of 151,936).
 SCORED_ROWS = 512
+# Sequences of a batch that `generate` makes, where it is not told.
+MAX_BATCH = 64
 # Batch sizes whose fixed metadata buffers are kept; the least recently used goes, with its graphs.
 MAX_DECODE_BATCH_SIZES = 96
 
@@ -437,7 +439,7 @@ class Engine:
                 if fed[i] == len(texts[i]) - 1:
                     del fed[i]
 
-    def generate(self, prompts, params=None, max_batch=64, on_token=None, interrupt=None, prefill_chunk=None):
+    def generate(self, prompts, params=None, max_batch=MAX_BATCH, on_token=None, interrupt=None, prefill_chunk=None):
         """Generate from lists of token ids; see engine.generate.Generator."""
         from .generate import Generator
         gen = Generator(self, max_batch=max_batch, prefill_chunk=prefill_chunk)

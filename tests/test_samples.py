@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from herbert_rs_amd.cache import FreeList
-from herbert_rs_amd.engine.generate import Generator, plan_batches
+from herbert_rs_amd.engine.generate import GenerationResult, Generator, plan_batches
 from herbert_rs_amd.errors import RequestError
 from herbert_rs_amd.sampling import SamplingParams
 
@@ -146,3 +146,71 @@ def test_answers_run_in_as_many_batches_as_there_are_slots_for(slots, held, chun
     for s in mine:
         engine.free_slot(s)
     assert engine.cache.slots.held_count == 0
+
+
+class Loaded:
+    """What `load` gave: how many tokens it was to hold, and which calls it got."""
+
+    def __init__(self):
+        self.room, self.asked = [], []
+
+    def __call__(self, model, dtype="bfloat16", cache_tokens=None, max_slots=None):
+        self.room.append(cache_tokens)
+        return self
+
+    def generate(self, prompts, params, **kw):
+        self.asked.append(params.samples)
+        return [GenerationResult([1], "length", len(p)) for p in prompts for _ in range(params.samples)]
+
+    def score(self, prompt, continuations, top):
+        return [[] for _ in continuations]
+
+
+def test_caches_are_as_large_as_what_runs_at_once(monkeypatch):
+    """A thousand answers in batches of 64 need the room of 64."""
+    from herbert_rs_amd import api
+    loaded = Loaded()
+    monkeypatch.setattr(api, "load", loaded)
+    for prompts, samples, max_batch in (([[1] * 200], 1000, 64), ([[1] * 200], 64, 64), ([[1] * 200] * 30, 7, 64), ([[1] * 200] * 300, 3, 16)):
+        out = api.generate("folder", prompts, max_tokens=100, samples=samples, max_batch=max_batch)
+        assert len(out) == len(prompts) and all(len(a) == samples for a in out)
+        room = loaded.room[-1]
+        biggest = max(batch_pages(b, [200] * len(prompts), 100, samples)
+                      for b in plan_batches([200] * len(prompts), 100, max_batch, 64 * 10 ** 6, 4096, samples))
+        assert 64 * biggest <= room <= 64 * (biggest + 4 * max_batch)
+    for n in (10, 512, 20000):
+        api.score("folder", [1] * 200, [[5] * 30] * n)
+        assert loaded.room[-1] <= 200 + 128 + 192 * min(n, 512)
+
+
+def batch_pages(members, lengths, max_new, samples):
+    """Pages that a batch holds at its end: a prompt's whole pages once."""
+    total = 0
+    for p in {i // samples for i in members}:
+        whole, count = -(-(lengths[p] + max_new) // 64), sum(i // samples == p for i in members)
+        total += whole + (count - 1) * (whole - lengths[p] // 64)
+    return total
+
+
+def test_wrong_parameters_are_refused_before_a_model_is_loaded(monkeypatch):
+    from herbert_rs_amd import api
+    loaded = Loaded()
+    monkeypatch.setattr(api, "load", loaded)
+    for bad in (dict(samples=0), dict(samples=-3), dict(temperature=-1.0)):
+        with pytest.raises(RequestError):
+            api.generate("folder", [[1, 2]], **bad)
+    assert loaded.room == []
+
+
+def test_the_command_line_asks_for_the_room_of_what_runs_at_once(monkeypatch, tmp_path):
+    from herbert_rs_amd import api, cli
+    from .tiny import make_folder
+    folder, asked = make_folder(tmp_path, "A"), []
+
+    def load(model, dtype, cache_tokens):
+        asked.append(cache_tokens)
+        raise RequestError("far enough")
+    monkeypatch.setattr(api, "load", load)
+    for samples in (1, 3, 64, 1000):
+        assert cli.main(["--model", folder, "--prompt", "5,17,3", "--max-tokens", "40", "--samples", str(samples)]) == 1
+    assert asked == [3 + 105, 3 + 105 + 2 * 232, 3 + 105 + 63 * 232, 3 + 105 + 63 * 232]
