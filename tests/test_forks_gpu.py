@@ -482,3 +482,23 @@ def test_forks_of_a_model_whose_scores_have_a_scale_that_is_not_positive(scale, 
     for i, w in enumerate(ways):
         ref = mefatar_tiny.plain_logits(str(tmp_path), prompt + w)
         assert all(close(rows[at][i], ref[75 + at], "float32", "mef", "turned scores")[0] for at in range(6))
+
+
+@pytest.mark.parametrize("graphs", [True, False])
+@pytest.mark.parametrize("family, name", [("mefatar", "Q"), ("mefatar", "W"), ("figalorn", "F"), ("figalorn", "R")])
+def test_forks_read_together_in_bfloat16(family, name, graphs, used, model_root):
+    """The families that choose no experts: forks whose shared pages are read together, against the plain implementation."""
+    tiny = importlib.import_module(f"tests.{family}_tiny")
+    compare = importlib.import_module(f"tests.test_{family}_gpu").compare
+    folder, vocab = tiny.make_folder(model_root, name, "bfloat16"), tiny.CONFIGS[name][0]["vocab"]
+    engine = hb.Engine.from_folder(folder, dtype="bfloat16", max_tokens=64 * 40, max_slots=8, use_graphs=graphs)
+    prompt, ways = random_tokens(vocab, 140, 1), [random_tokens(vocab, 60, 30 + i) for i in range(4)]
+    first = engine.alloc_slot()
+    engine.step([StepEntry(first, prompt, [])])
+    slots = [first] + engine.fork(first, 3)
+    rows = [engine.step([StepEntry(s, [w[at]], [0]) for s, w in zip(slots, ways)]).cpu().numpy() for at in range(60)]
+    assert len(used) > (0 if graphs else 50)
+    for i, w in enumerate(ways):
+        bound = {"bound": "figfar"} if (family, name) == ("figalorn", "F") else {}
+        compare([r[i] for r in rows], folder, prompt + w, range(140, 200), "bfloat16", f"{name} forks read together", **bound)
+    engine.cache.check()

@@ -274,3 +274,40 @@ def test_calls_refused_before_a_launch(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: 5)
     with pytest.raises(BackendError, match="tensors lie on GPUs .0., the current one is 5"):
         shared.attention(q, meta, kv, out, 4, 2, 64, 0.125)
+
+
+def chains(weight, q, kv, table, held, news, nq, nkv, hd):
+    """What float32 results may be off by, counted along the kernel's own chains as a walk of independent roundings, each evenly within u = 2^-24 (half
+    a step) of its value, whose square root of the sum of squares is taken six times.
+    A score is four sums side by side of n = 16 ceil(hd / 64) products each: a sum of random signs is as large as the root of the sum of its products'
+    squares, r, at most, so 6 sqrt(n) u r / sqrt(3); the sums of sums, the scale, the difference from the reference, the exponential and the
+    factors of a page and of an item are eight further roundings of u (1 + 2 |score|). A weight is off by as much of itself, numerator and
+    denominator: twice that. The products with values: chains of 32, a sum and a rescaling a page and an item (no more than pages), numerator and
+    denominator: 2 x 6 sqrt(34 + 4 pages) u / sqrt(3)."""
+    out = torch.empty_like(weight[..., 0])
+    k, q, row = kv.k.cpu().double(), q.cpu().double().view(-1, nq, hd), 0
+    for i, (before, n) in enumerate(zip(held, news)):
+        keys = k[torch.from_numpy(table[i, :-(-(before + n) // 64)].astype(np.int64))].permute(1, 0, 2, 3).reshape(nkv, -1, hd)
+        pages = (before + n) // 64 + 1
+        for t in range(row, row + n):
+            for h in range(nq):
+                seen = keys[h // (nq // nkv), :before + t - row + 1]
+                r = (seen.square() @ q[t, h].square()).max().sqrt() * hd ** -0.5
+                top = (seen @ q[t, h]).abs().max() * hd ** -0.5
+                out[t, h] = 2 * (6 * (16 * -(-hd // 64) / 3) ** 0.5 * r + 8 * (1 + 2 * top)) + 2 * 6 * ((34 + 4 * pages) / 3) ** 0.5
+        row += n
+    return 2.0 ** -24 * out[..., None] * weight + 1e-30
+
+
+@pytest.mark.parametrize("seqs, held, news, nq, nkv, hd", [
+    (plain_samples(9, 5), [64 * 5 + 5 * i for i in range(9)], [1] * 9, 8, 2, 128),
+    (plain_samples(5, 40, 2), [64 * 40 + 9 + i for i in range(5)], [1] * 5, 4, 2, 64),
+    (plain_samples(4, 3, 2), [192, 200, 230, 192], [40, 7, 64, 1], 4, 2, 80),
+    (plain_samples(3, 2), [130, 150, 190], [1] * 3, 2, 1, 256)])
+def test_float32_results_lie_within_the_roundings_of_their_chains(seqs, held, news, nq, nkv, hd):
+    q, meta, kv, out, table = run(seqs, held, news, nq, nkv, hd, F32, seed=7)
+    want, weight, _ = reference(q, kv, table, held, news, nq, nkv, hd, hd ** -0.5)
+    allowed = chains(weight, q, kv, table, held, news, nq, nkv, hd)
+    share = ((out.cpu().double().view(want.shape) - want).abs() / allowed).max().item()
+    observe("shared attention f32 of its chains' roundings", share)
+    assert share <= 1.0
