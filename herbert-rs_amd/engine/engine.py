@@ -166,7 +166,7 @@ class Engine:
     def fork(self, slot, count=1):
         """`count` new slots that hold what `slot` holds, without a pass through the model: they share its pages of keys and values
         (a page is copied when one of its holders writes into it) and have copies of its fixed-size state. Where slots of one step
-        share pages, an attention that sees whole contexts reads those once for all of them. The reference has one cache a sequence
+        share pages, an attention that sees whole contexts reads those once for all of them where that ends sooner. The reference has one cache a sequence
         and runs a prompt again for every answer to it (crates/backends/backend_common/src/kv_cache.rs:270-273)."""
         return self.cache.fork(slot, count)
 
@@ -377,7 +377,8 @@ class Engine:
         """What the model says of given continuations of a prompt: for each a list with a sampling.logprobs.TokenLogprob a token
         (log p(token | prompt, the continuation's tokens before it), the entropy there and the `top` most probable tokens).
         The prompt goes through the model once; the continuations go on from forks of its slot, as many side by side as there
-        are slots for, and their steps read the prompt's keys and values together. A text by itself: its first token as the
+        are slots for. Their steps read the prompt's keys and values together where that ends sooner (kernels.shared.pays: in bfloat16 up to
+        8 tokens a sequence, that is 64 long continuations or more side by side, in float32 up to 200). A text by itself: its first token as the
         prompt, the rest as the continuation."""
         from ..sampling import MOST_ALTERNATIVES
         from ..sampling.logprobs import LogprobReader

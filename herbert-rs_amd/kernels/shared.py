@@ -23,13 +23,13 @@ ITEM_INTS = 8
 COLUMNS = {torch.bfloat16: 128, torch.float32: 16}      # (row, head) pairs of a kv head that an item holds at most
 F32_MOST_DIM = 256
 # Workgroups that a step is cut into: as many as the GPU holds at a time, two a CU in bfloat16, four in float32. Measured with 256, 384 and 512 in
-# bfloat16: 128 answers to 32,768 tokens 110, 95 and 89 us, 64 to 8,192 37, 33 and 33 us, 12 continuations of a text of 2,000 tokens
-# 46, 44 and 46 us.
+# bfloat16, one call after another over the same pages (caches warm; with cold ones 97 and 38 us of the first two at 512): 128 answers to 32,768 tokens 110, 95
+# and 89 us, 64 to 8,192 37, 33 and 33 us, 12 continuations of a text of 2,000 tokens 46, 44 and 46 us.
 WORKGROUPS = {torch.bfloat16: 512, torch.float32: 1024}
 OPERANDS = ("q", "out", "key pages", "value pages", "page_table", "positions", "seq_of", "slots", "sinks")
 MASKED_COLUMNS = 64             # of an item in whose pages are places that some of its rows see and others do not: the wide ones ask no mask
 # Pages of the longest sequence up to which every sequence is an item of its own, whose pages four waves of one CU read (at 40 bytes a nanosecond), and nothing
-# is joined. 2, 8 and 64 sequences of 4, 8 and 8 kv heads of 128: of 4 pages 8.0, 8.1, 12.0 us by themselves, 10.1, 11.3, 15.3 joined; of 6 9.2, 9.4, 15.5 and 11.0, 11.8,
+# is joined. Caches warm, 2, 8 and 64 sequences of 4, 8 and 8 kv heads of 128: of 4 pages 8.0, 8.1, 12.0 us by themselves, 10.1, 11.3, 15.3 joined; of 6 9.2, 9.4, 15.5 and 11.0, 11.8,
 # 15.9; of 8 10.5, 10.8, 18.5 and 10.9, 11.8, 16.6.
 BY_ITSELF_PAGES = 6
 # The attention of one sequence after another also normalizes, rotates and writes what the projection gave; before the shared one that is a kernel of its
@@ -51,9 +51,11 @@ SAVED_SEQUENCES = 20
 ALONE_DIM = 64
 ALONE_PAIRS = 64
 ALONE_PAGES = 3
-# Tokens a sequence from which a step is worth more as a prompt: its own columns fill the products by then. 24 sequences of 8, 40 and 200 new tokens behind
-# 2,000 shared ones: 28, 46, 157 us shared, 34, 38, 121 us separate; behind 1,000: 23, 40, 128 and 23, 27, 80 us. In float32 16 sequences of 8, 40 and
-# 200 behind 256: 15, 38, 135 us shared, 21, 33, 129 us separate; behind 2,000: 37, 128, 526 and 98, 146, 566 us.
+# New tokens a sequence, on the mean, up to which a step is taken: beyond, its own columns fill the products. Microseconds shared / separate. bfloat16, 32 heads
+# of 128 over 8: 24 sequences of 4, 8, 12, 16 and 40 tokens behind 2,000 29/33, 30/33, 33/33, 39/34, 62/68, of 200 297/196; 64 behind 1,000 28/42, 33/43, 44/45, 50/47,
+# 114/80; behind 4,000, where more is saved, 24 sequences 27/59, 35/58, 40/59, 50/61, 88/122. float32, 16 sequences of 16, 40, 80 and 200 tokens: 16 heads of 128
+# over 8 behind 256 27/22, 49/48, 91/83, 239/216, behind 2,000 87/100, 198/227, 378/364, 947/921; 32 over 8 behind 2,000 159/146, 378/358, 741/700, 1,875/1,760; 8 of 64 over 2
+# behind 256 12/15, 17/19, 27/25, 58/60, behind 2,000 28/65, 54/87, 97/115, 235/262; 8 sequences of 1, 8 and 40, 8 of 256 over 4, behind 2,000 18/527, 53/532, 151/529.
 MANY_TOKENS = {torch.bfloat16: 8, torch.float32: 200}
 
 
