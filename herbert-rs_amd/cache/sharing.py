@@ -34,6 +34,11 @@ class SharedPages:
         return self._filled
 
     @cached_property
+    def node_array(self):
+        """The nodes as one array [nodes, 4]."""
+        return np.ascontiguousarray(np.array(self.nodes, dtype=np.int64).reshape(-1, 4))
+
+    @cached_property
     def pages_saved(self):
         """How many pages fewer are read than if every sequence read its own."""
         return sum((count - 1) * (end - page) for _, count, page, end in self.nodes if count > 1)

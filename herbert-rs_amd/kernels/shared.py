@@ -4,6 +4,7 @@ checks, the launch (csrc/attention_shared.hip).
 The reference attends over every sequence's cache by itself
 (crates/backends/backend_common/src/attention_common.rs:20-124)."""
 import ctypes
+from functools import lru_cache
 
 import numpy as np
 import torch
@@ -68,13 +69,6 @@ def supported(kv, nq, nkv, hd, dtype):
     return dtype == torch.float32 and hd % 4 == 0 and 0 < hd <= F32_MOST_DIM
 
 
-def _even(first, end, most):
-    """Cut first .. end into as few stretches of at most `most` as there can be, alike in length: (first, length)."""
-    count = -(-(end - first) // most)
-    cuts = [first + (end - first) * i // count for i in range(count + 1)]
-    return [(a, b - a) for a, b in zip(cuts[:-1], cuts[1:])]
-
-
 def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=1):
     """How a step is cut up. starts: the first packed row of each sequence and the last one's end; context: the positions it
     holds after the step; slots: theirs; sharing: a SharedPages. Returns int32 arrays (items [n, 8], order [rows], part_start
@@ -82,66 +76,26 @@ def plan(starts, context, slots, sharing, group, nkv, columns, workgroups, grid=
 
     A node of the sharing is cut into tiles of as many rows as fit `columns`; a tile's pages are cut into ranges of about as many pages
     each that the workgroups (items x kv heads) come to `workgroups`, whole rounds of the waves that take them in turn. The pages
-    that a tile of more than 64 columns sees in part are items of their own."""
-    starts, context = np.asarray(starts, dtype=np.int64), np.asarray(context, dtype=np.int64)
-    counts = np.diff(starts)
-    if len(sharing.order) != len(counts):
-        raise BackendError(f"shared attention: pages shared by {len(sharing.order)} sequences in a step of {len(counts)}")
-    row_of = np.concatenate([[0], np.cumsum(counts[sharing.order])])            # a sequence's first row in the order
-    of_row = np.repeat(sharing.order, counts[sharing.order])                    # whose row it is
-    order = starts[of_row] + np.arange(len(of_row)) - row_of[np.repeat(np.arange(len(counts)), counts[sharing.order])]
-    tall = max(1, columns // group)
-    short = max(1, MASKED_COLUMNS // group) if columns == 128 else tall
-    tiles = []                                                                  # row0, rows, sequence, first page, end, first page seen in part
-    nodes = np.array(sharing.nodes, dtype=np.int64).reshape(-1, 4)
-    alone = (nodes[:, 3] < 0) & (counts[sharing.order[nodes[:, 0]]] == 1)       # a sequence's own pages, one row: all of them at once
-    for first, count, page, end in nodes[~alone].tolist():
-        a, b, seq = int(row_of[first]), int(row_of[first + count]), int(sharing.order[first])
-        for r, n in _even(a, b, tall):
-            if end >= 0:
-                tiles.append((r, n, seq, page, end, end))
-                continue
-            # A sequence's own rows: all of them see what lies before the first row's page; a tile ends at the page of its last row.
-            whole, page_from = (int(context[seq]) - (b - r)) // 64, page
-            if n * group > 64 and whole > page:
-                tiles.append((r, n, seq, page, whole, whole))
-                page_from = whole
-            for u, m in _even(r, r + n, short):
-                first_seen, last_seen = int(context[seq]) - (b - u), int(context[seq]) - (b - (u + m)) - 1
-                tiles.append((u, m, seq, page_from, last_seen // 64 + 1, first_seen // 64))
-    first = nodes[alone, 0]
-    seen = (context[sharing.order[first]] - 1) // 64
-    of_one = np.stack([row_of[first], np.ones_like(first), sharing.order[first], nodes[alone, 2], seen + 1, seen])
-    row0, rows, seq, page, end, whole = np.concatenate([np.array(tiles, dtype=np.int64).reshape(-1, 6).T, of_one], axis=1)
-    cols, pages = rows * group, end - page
-    turns = np.where(cols <= 32, 4, np.where(cols <= 64, 2, 1)) if columns == 128 else np.ones_like(cols)
-    share = max(1, -(-int(pages.sum()) * nkv // workgroups))
-    per = -(-share // turns) * turns
-    ranges = -(-pages // per)
-    per = -(-(-(-pages // ranges)) // turns) * turns
-    of = np.repeat(np.arange(len(rows)), ranges)
-    nth = np.arange(len(of)) - np.repeat(np.cumsum(ranges) - ranges, ranges)
-    items = np.zeros((len(of), ITEM_INTS), dtype=np.int64)
-    items[:, 0], items[:, 1], items[:, 2] = row0[of], rows[of], np.asarray(slots, dtype=np.int64)[seq[of]]
-    items[:, 3] = page[of] + nth * per[of]
-    items[:, 4] = np.minimum(items[:, 3] + per[of], end[of])
-    items[:, 6] = items[:, 4] > whole[of]
-    items = items[items[:, 4] > items[:, 3]]              # (ranges rounded up may leave the last ones nothing)
-    n = items[:, 1]
-    items[:, 5] = np.cumsum(n) - n
-    # a row's partial results lie side by side, in the order of its pages
-    total = int(n.sum())
-    row = np.repeat(items[:, 0] - items[:, 5], n) + np.arange(total)
-    parts = np.empty(total, dtype=np.int64)
-    parts[np.argsort(row, kind="stable")] = np.arange(total)
-    part_start = np.concatenate([[0], np.cumsum(np.bincount(row, minlength=len(order)))])
-    # the longest items first, those over the same pages side by side
-    items = items[np.lexsort((items[:, 0], items[:, 3], items[:, 3] - items[:, 4]))]
-    most = int(n.max())
-    n_items = -(-len(items) // grid) * grid
-    items = np.concatenate([items, np.zeros((n_items - len(items), ITEM_INTS), dtype=np.int64)])
-    as32 = lambda x: np.ascontiguousarray(x, dtype=np.int32)
-    return as32(items), as32(order), as32(part_start), as32(parts), most
+    that a tile of more than 64 columns sees in part are items of their own.
+
+    Cut natively (csrc/hostcall.cpp): steps of many sequences begin a page nearly every time, and models whose steps wait for the host waited for
+    NumPy. 128 forks of 2,000 tokens, one layer 560 us a step, now 450 (410 with every sequence reading its own pages), four layers 562, now 503 (755)."""
+    numbers, n_items, _, most = _cut(starts, context, slots, sharing, group, nkv, columns, workgroups, grid)
+    rows = int(starts[-1])
+    at = np.cumsum([ITEM_INTS * n_items, rows, rows + 1])
+    return numbers[:at[0]].reshape(n_items, ITEM_INTS), numbers[at[0]:at[1]], numbers[at[1]:at[2]], numbers[at[2]:], most
+
+
+def _cut(starts, context, slots, sharing, group, nkv, columns, workgroups, grid, room=0):
+    """What `plan` gives, one behind the other, the items in the room of `room` at least; how many items and parts, the most rows of an item."""
+    if len(sharing.order) != len(starts) - 1:
+        raise BackendError(f"shared attention: pages shared by {len(sharing.order)} sequences in a step of {len(starts) - 1}")
+    as64 = lambda x: np.ascontiguousarray(x, dtype=np.int64)
+    made = lib.host().plan(as64(starts), as64(context), as64(slots), as64(sharing.order), sharing.node_array, group, nkv, columns, MASKED_COLUMNS,
+                           workgroups, grid, room)
+    if made is None:
+        raise BackendError("shared attention: the pages that are said to be shared are not those of this step's sequences, each in its place")
+    return (np.frombuffer(made[0], dtype=np.int32), *made[1:])
 
 
 def _by_itself(meta, nkv, dtype):
@@ -150,24 +104,28 @@ def _by_itself(meta, nkv, dtype):
             and int(meta.host_context.max()) <= 64 * BY_ITSELF_PAGES)
 
 
-def _planned(meta, group, nkv, dtype, grid=1):
-    """(What `plan` gives, whether every row is one item's.)"""
+@lru_cache(maxsize=64)
+def _all_alone(n):
+    return SharedPages(np.arange(n), [(i, 1, 0, -1) for i in range(n)])
+
+
+def _planned(meta, group, nkv, dtype, cut, *grid_and_room):
+    """(What `cut`, that is `plan` or `_cut`, gives of a step, whether every row is one item's.)"""
     sharing, workgroups, direct = meta.shared, WORKGROUPS[dtype], _by_itself(meta, nkv, dtype)
     if direct:
-        n = len(sharing.order)
-        sharing, workgroups = SharedPages(np.arange(n), [(i, 1, 0, -1) for i in range(n)]), 1
-    return (*plan(meta.host_starts, meta.host_context, meta.host_slots, sharing, group, nkv, COLUMNS[dtype], workgroups, grid), direct)
+        sharing, workgroups = _all_alone(len(sharing.order)), 1
+    return (*cut(meta.host_starts, meta.host_context, meta.host_slots, sharing, group, nkv, COLUMNS[dtype], workgroups, *grid_and_room), direct)
 
 
 class Plan:
     """A plan on the GPU: of meta.shared as it is now."""
 
     def __init__(self, meta, group, nkv, dtype):
-        items, order, part_start, parts, self.max_rows, self.direct = _planned(meta, group, nkv, dtype)
-        both = send(np.concatenate([a.ravel() for a in (items, order, part_start, parts)]), meta.positions.device)
-        at = np.cumsum([a.size for a in (items, order, part_start, parts)])
-        self.items, self.order, self.part_start, self.parts = both[:at[0]], both[at[0]:at[1]], both[at[1]:at[2]], both[at[2]:]
-        self.sharing, self.n_items, self.n_parts = meta.shared, len(items), len(parts)
+        numbers, self.n_items, self.n_parts, self.max_rows, self.direct = _planned(meta, group, nkv, dtype, _cut, 1)
+        at = np.cumsum([ITEM_INTS * self.n_items, meta.num_tokens, meta.num_tokens + 1])
+        b = send(numbers, meta.positions.device)
+        self.items, self.order, self.part_start, self.parts = b[:at[0]], b[at[0]:at[1]], b[at[1]:at[2]], b[at[2]:]
+        self.sharing = meta.shared
 
 
 class StaticPlan:
@@ -198,20 +156,18 @@ class StaticPlan:
         before = self._filled_for
         if before is not None and before[0] is meta.shared and before[1:] == filled_for[1:]:
             return
-        items, order, part_start, parts, _, self.direct = _planned(meta, self.group, self.nkv, self.dtype, self.GRID)
-        self.n_items, self.n_parts = len(items), 1 << (len(parts) - 1).bit_length()
-        if len(items) > self._rooms[0] or len(parts) > self._rooms[1]:
+        numbers, self.n_items, n_parts, _, self.direct = _planned(meta, self.group, self.nkv, self.dtype, _cut, self.GRID, self._rooms[0])
+        self.n_parts = 1 << (n_parts - 1).bit_length()
+        if self.n_items > self._rooms[0] or n_parts > self._rooms[1]:
             if self._buffer is not None:
                 self._outgrown.append(self._buffer)
-            self._rooms = (2 * len(items), 2 * len(parts))
-            self._buffer = torch.zeros(ITEM_INTS * self._rooms[0] + 2 * self.rows + 1 + self._rooms[1], dtype=torch.int32, device=self.device)
+            self._rooms = (2 * self.n_items, 2 * n_parts)
+            at = np.cumsum([ITEM_INTS * self._rooms[0], self.rows, self.rows + 1, self._rooms[1]])
+            b = self._buffer = torch.zeros(at[3], dtype=torch.int32, device=self.device)
+            self.items, self.order, self.part_start, self.parts = b[:at[0]], b[at[0]:at[1]], b[at[1]:at[2]], b[at[2]:]
             self.made += 1
-        at = np.cumsum([ITEM_INTS * self._rooms[0], self.rows, self.rows + 1, self._rooms[1]])
-        b = self._buffer
-        self.items, self.order, self.part_start, self.parts = b[:at[0]], b[at[0]:at[1]], b[at[1]:at[2]], b[at[2]:]
-        host = np.zeros(at[2] + len(parts), dtype=np.int32)
-        host[:items.size], host[at[0]:at[1]], host[at[1]:at[2]], host[at[2]:] = items.ravel(), order, part_start, parts
-        send_into(host, b[:len(host)])
+            numbers = _planned(meta, self.group, self.nkv, self.dtype, _cut, self.GRID, self._rooms[0])[0]
+        send_into(numbers, self._buffer[:len(numbers)])
         self._filled_for = filled_for
 
 

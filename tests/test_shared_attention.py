@@ -12,7 +12,7 @@ from herbert_rs_amd.engine import Model, StepEntry, batch
 from herbert_rs_amd.errors import BackendError
 from herbert_rs_amd.kernels import lib, shared
 
-from . import figalorn_tiny
+from . import figalorn_tiny, plan_oracle
 from .shared_util import tables
 from .tiny import spec_of
 
@@ -263,7 +263,7 @@ def test_short_contexts_behind_a_kernel_of_their_own_are_read_sequence_by_sequen
     assert shared.worth_over([KVNeed(nkv, hd)], torch.bfloat16)(meta) == (False,)
     if taken:
         meta.host_starts, meta.host_slots = np.arange(count + 1), np.arange(count)
-        items, order, part_start, parts, most, direct = shared._planned(meta, 4, nkv, torch.bfloat16)
+        items, order, part_start, parts, most, direct = shared._planned(meta, 4, nkv, torch.bfloat16, shared.plan)
         assert direct and len(items) == count and most == 1
 
 
@@ -283,3 +283,54 @@ def test_scores_with_a_scale_that_is_not_positive_stay_with_the_ordinary_attenti
     mixer = Model(spec_of(raw)[1]).blocks[1].mixer.sides[0]
     ctx = SimpleNamespace(meta=decode_of(4, 2, 130), rt=SimpleNamespace(dtype=torch.float32))
     assert mixer._shares(ctx, cache_of(mixer.nkv, mixer.hd, torch.float32)) == taken
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_the_plan_is_that_of_the_formulas(seed):
+    """The host's native cut against the same one in NumPy, number for number: random trees, single tokens and several, padding, shapes of graphs."""
+    rng = np.random.default_rng(1000 + seed)
+    table, held, news = random_step(rng)
+    found = shared_pages(table, held)
+    if found is None:
+        found = SharedPages(np.arange(len(held)), [(i, 1, 0, -1) for i in range(len(held))])
+    starts, context = np.concatenate([[0], np.cumsum(news)]), [h + n for h, n in zip(held, news)]
+    for columns, group, nkv, workgroups, grid in ((128, 4, 8, 512, 1), (128, 1, 2, 512, 16), (128, 32, 1, 1, 16), (128, 7, 4, 100000, 1), (16, 2, 4, 1024, 16),
+                                                  (16, 16, 1, 7, 1), (16, 24, 2, 1024, 1)):
+        args = starts.astype(np.int32), np.array(context, dtype=np.int32), rng.permutation(len(held)), found, group, nkv, columns, workgroups, grid
+        got, want = shared.plan(*args), plan_oracle.plan(*args)
+        assert all(g.dtype == np.int32 and g.shape == w.shape and (g == w).all() for g, w in zip(got[:4], want[:4])) and got[4] == want[4]
+
+
+@pytest.mark.parametrize("change, text", [
+    (dict(nodes=[(0, 3, 0, 2), (0, 1, 2, -1), (1, 1, 2, -1)]), "each in its place"),              # a sequence's own pages are nowhere
+    (dict(nodes=[(0, 3, 0, 2), (0, 1, 2, -1), (1, 1, 3, -1), (2, 1, 2, -1)]), "each in its place"),          # a page is left out
+    (dict(nodes=[(0, 3, 0, 2), (0, 1, 1, -1), (1, 1, 2, -1), (2, 1, 2, -1)]), "each in its place"),          # or there twice
+    (dict(nodes=[(0, 3, 0, 3), (0, 1, 3, -1), (1, 1, 3, -1), (2, 1, 3, -1)]), "each in its place"),          # beyond what is held before the step
+    (dict(nodes=[(0, 4, 0, 2), (0, 1, 2, -1), (1, 1, 2, -1), (2, 1, 2, -1)]), "each in its place"),
+    (dict(nodes=[(0, 3, 0, 2), (0, 1, 2, -1), (1, 1, 2, -1), (1 << 40, 1, 2, -1)]), "each in its place"),
+    (dict(nodes=[(0, 3, -1, 2), (0, 1, 2, -1), (1, 1, 2, -1), (2, 1, 2, -1)]), "each in its place"),
+    (dict(order=[0, 1, 1]), "each in its place"), (dict(order=[0, 1, 3]), "each in its place"), (dict(order=[0, 1]), "shared by 2 sequences"),
+    (dict(context=[140, 0, 150]), "each in its place"), (dict(starts=[0, 1, 1, 2]), "each in its place")])
+def test_pages_that_are_not_those_of_the_step_are_refused(change, text):
+    args = dict(starts=[0, 1, 2, 3], context=[140, 131, 150], slots=[5, 3, 4], order=[0, 1, 2],
+                nodes=[(0, 3, 0, 2), (0, 1, 2, -1), (1, 1, 2, -1), (2, 1, 2, -1)])
+
+    def cut(starts, context, slots, order, nodes):
+        return shared.plan(starts, context, slots, SharedPages(np.array(order), nodes), 4, 8, 128, 512)
+    assert len(cut(**args)[0]) >= 4
+    with pytest.raises(BackendError, match=text):
+        cut(**dict(args, **change))
+
+
+def test_the_native_plan_takes_integers_of_64_bits_alone():
+    good = [np.array([0, 1]), np.array([5]), np.array([0]), np.array([0]), np.array([[0, 1, 0, -1]])]
+    numbers = (4, 8, 128, 64, 512, 1, 0)
+    assert lib.host().plan(*good, *numbers)[1] == 1
+    for i in range(5):
+        for bad in (good[i].astype(np.int32), good[i].astype(np.float64), [0, 1], None):
+            with pytest.raises(TypeError):
+                lib.host().plan(*good[:i], bad, *good[i + 1:], *numbers)
+    with pytest.raises(TypeError):
+        lib.host().plan(*good, *numbers[:-1])
+    for i in range(6):
+        assert lib.host().plan(*good, *(n if j != i else 0 for j, n in enumerate(numbers))) is None
