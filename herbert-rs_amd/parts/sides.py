@@ -64,7 +64,7 @@ class SideBySide(Part):
         return needs or None
 
     def heads_prepared_alone(self):
-        return tuple(h for m in self.sides for h in m.heads_prepared_alone())
+        return tuple(h for m in self.sides for h in getattr(m, "heads_prepared_alone", tuple)())
 
     def load(self, tensors, rt):
         for m in self.sides:
