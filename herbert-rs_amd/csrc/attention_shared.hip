@@ -39,7 +39,7 @@ struct Item {
 // 256 registers and 68 KB of LDS: two workgroups a CU, so that items that wait for memory and items that compute overlap.
 // Scores, exponentials, their sums and the outputs are float32. An exponential is rounded to bfloat16 (2^-8 of itself at most) before it meets its value, since the products
 // take bfloat16 alone, and a head and a rest of it would double the second half of the matrix work; its sum is that of the unrounded ones. Against 64 bits results
-// are off by 0.0020 to 0.0023 of their root mean square, where the exact ones rounded to bfloat16 are by 0.0017. No sum's order changes: the same call gives the same bits.
+// are off by 0.0017 to 0.0023 of their root mean square, where the exact ones rounded to bfloat16 are by 0.0017. No sum's order changes: the same call gives the same bits.
 // 8/32 heads of 128, microseconds (join apart, caches warm; cold, join and all: 97, 38, 23.4 and 14.5): 128 answers to 32,768 tokens 86 to 92 (0.75 PFLOP/s; the products are 39 % of the time and the softmax's vector
 // work 37 %, partly side by side; with 64 columns a wave 120, since registers were moved between files), 64 to 8,192 29 (108 MB at 3.7 TB/s), 48 questions
 // behind 6 texts 20.6 (82 MB at 4.0 TB/s), 8 answers to 4,096 10.4, where a page a wave is a chain of loads. The first form, every item
